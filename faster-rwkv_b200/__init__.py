@@ -22,7 +22,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FR_B200_LIB") or os.path.join(_HERE, "csrc", "libfr_b200.so")
 
 W_FP16, W_INT8, W_INT4 = 0, 1, 2
-T_F16, T_F32 = 0, 1
+T_F16, T_F32, T_BF16 = 0, 1, 2
 _VERSIONS = {"4": 4, "5": 50, "5.0": 50, "5.1": 51, "5.2": 52}
 _FORMATS = {"fp16": W_FP16, "int8": W_INT8, "int4": W_INT4}
 
@@ -50,7 +50,7 @@ class Info(ctypes.Structure):
 _lib: Optional[ctypes.CDLL] = None
 
 # name -> (restype, argtypes); every symbol include/fr_b200.h declares
-_vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_vp, _i, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 SIGNATURES = {
     "fr_b200_create": (_i, [ctypes.POINTER(Config), ctypes.POINTER(_vp)]),
     "fr_b200_set_tensor": (_i, [_vp, ctypes.c_char_p, _vp, _i, ctypes.POINTER(ctypes.c_int64), _i]),
@@ -92,6 +92,16 @@ SIGNATURES = {
     "fr_b200_groupnorm": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "fr_b200_elementwise": (_i, [_i, _vp, _i, _vp, _i, _vp, _i, ctypes.c_float, _vp, _i, _sz, _vp]),
     "fr_b200_matmul": (_i, [_vp, _i, _i, _i, _vp, _i, _i, _vp, _i, _i, _vp]),
+    "fr_b200_linear": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i, _i, _vp, _i, _vp, _i64, _vp, _i64, _i, _i, _vp]),
+    "fr_b200_conv_seq": (_i, [_vp, _i64, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
+    "fr_b200_conv_step": (_i, [_vp, _i64, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
+    "fr_b200_ssm_seq_workspace": (_sz, [_i64, _i, _i, _i]),
+    "fr_b200_ssm_seq": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i, _i, _i64, _i, _i, _i, _vp, _i,
+                             _vp, _i64, _i, _vp, _vp, _vp, _i64, _vp, _sz, _i, _vp]),
+    "fr_b200_ssm_step": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i, _i, _i, _i, _i, _i,
+                              _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
+    "fr_b200_slots_copy": (_i, [_vp, _sz, _sz, _i, _i, _vp, _vp, _i, _vp]),
+    "fr_b200_state_copy": (_i, [_vp, _i, _vp, _vp, _vp]),
     "fr_b200_op_last_error": (ctypes.c_char_p, []),
     "fr_b200_strerror": (ctypes.c_char_p, [_i]),
     "fr_b200_last_error": (ctypes.c_char_p, []),
@@ -257,6 +267,15 @@ class Model:
     def reset_states(self, slot: int = -1) -> None:
         check(lib().fr_b200_state_reset(self._h, slot), "fr_b200_state_reset")
 
+    def copy_states(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Slot dst[i] takes the state that slot src[i] has before the call (src -1: the initial state), on the device:
+        fork a prompt's state into several streams, reorder the streams of a beam search, close the gaps that finished
+        streams leave.  Every slot appears in dst once at most."""
+        s, d = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+        if s.shape != d.shape or s.ndim != 1:
+            raise ValueError("src and dst are two lists of as many slots")
+        check(lib().fr_b200_state_copy(self._h, len(s), _np_ptr(s), _np_ptr(d), None), "fr_b200_state_copy")
+
     def states(self, slot: int = 0) -> List[List[np.ndarray]]:
         """Per layer the 5 (RWKV-4) or 3 (RWKV-5) state tensors, shapes and dtypes of model.cpp:145-177."""
         L = lib()
@@ -414,3 +433,7 @@ def matvec(W: np.ndarray, x: np.ndarray, weight_format: int, device: int = 0) ->
     y = np.empty((B, N), np.float32)
     check(lib().fr_b200_matvec(_np_ptr(W), K, N, weight_format, _np_ptr(x), B, _np_ptr(y), device), "fr_b200_matvec")
     return y
+
+
+# operators of a recurrent layer over torch CUDA tensors
+from .ops import conv_seq, conv_step, copy_slots, linear, ssm_seq, ssm_step  # noqa: E402,F401

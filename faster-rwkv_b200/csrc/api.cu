@@ -11,6 +11,7 @@
 
 #include "../../include/fr_b200.h"
 #include "internal.h"
+#include "operators.cuh"
 
 using namespace frb;
 
@@ -1533,6 +1534,27 @@ int fr_b200_state_import(fr_b200_model *m, int slot, const void *src, size_t src
   CU(cudaSetDevice(m->device));
   CU(cudaDeviceSynchronize());
   return state_copy(m, slot, const_cast<uint8_t *>(static_cast<const uint8_t *>(src)), false);
+}
+
+int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_t *dst, void *stream) {
+  if (!m) return fail(FR_B200_E_ARG, "null model");
+  if (!m->finalized) return fail(FR_B200_E_STATE, "state_copy before finalize");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  try {
+    if (int rc = check_moves(m->cfg.max_batch, n, src, dst)) return fail(rc, fr_b200_op_last_error());
+    if (capturing(st)) return fail(FR_B200_E_STATE, "state_copy on a capturing stream: which copy of its token-shift states a slot reads is kept on the host");
+    CU(cudaSetDevice(m->device));
+    // both copies of the token-shift states move, and with them which one is read next
+    std::vector<unsigned> par(m->par);
+    const SlotFill pp{off_mid(m->C, m->cfg.act_fp16) + 2 * (size_t)m->C * 4, m->layer_stride, m->L, m->C, -1e30f};
+    CU(launch_slots_copy(m->d_state, m->layer_stride * m->L, m->state_stride, m->cfg.max_batch, n, src, dst, m->v5 ? nullptr : &pp, st));
+    for (int i = 0; i < n; ++i) par[dst[i]] = src[i] < 0 ? 0u : m->par[src[i]];
+    m->par.swap(par);
+    if (m->cfg.host_visible_state) CU(cudaStreamSynchronize(st));
+  } catch (const std::bad_alloc &) {
+    return fail(FR_B200_E_NOMEM, "out of host memory");
+  }
+  return FR_B200_OK;
 }
 
 // ---- quantisers -----------------------------------------------------------------------------------

@@ -1,0 +1,163 @@
+// What the operators over device tensors share: element types, errors, the caller's device, checks of rows and slots,
+// and the tables of sequences and slots that travel with a launch.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <new>
+#include <string>
+#include <type_traits>
+#include <utility>
+#include <vector>
+
+#include "../../include/fr_b200.h"
+
+namespace frb {
+
+// status + text for fr_b200_op_last_error()
+int op_fail(int code, const std::string &msg);
+#define OP_CU(call)                                                                                               \
+  do {                                                                                                            \
+    cudaError_t e_ = (call);                                                                                      \
+    if (e_ != cudaSuccess) return frb::op_fail(FR_B200_E_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
+  } while (0)
+#define OP_REQUIRE(cond, msg)                                            \
+  do {                                                                   \
+    if (!(cond)) return frb::op_fail(FR_B200_E_ARG, msg);                 \
+  } while (0)
+// nothing is thrown across the C ABI
+#define OP_TRY try {
+#define OP_CATCH                                                                          \
+  }                                                                                       \
+  catch (const std::bad_alloc &) { return FR_B200_E_NOMEM; }                              \
+  catch (...) { return FR_B200_E_ARG; }
+
+// The call's device is current inside the call and the caller's again behind it.
+struct DeviceScope {
+  int before = -1;
+  cudaError_t enter(int device) {
+    cudaError_t e = cudaGetDevice(&before);
+    if (e != cudaSuccess) { before = -1; return e; }
+    if (before == device) { before = -1; return cudaSuccess; }
+    e = cudaSetDevice(device);
+    if (e != cudaSuccess) before = -1;
+    return e;
+  }
+  ~DeviceScope() { if (before >= 0) cudaSetDevice(before); }
+};
+
+// ---- elements ----
+inline int dt_bytes(int dt) { return dt == FR_B200_T_F32 ? 4 : 2; }
+inline bool dt_known(int dt) { return dt == FR_B200_T_F16 || dt == FR_B200_T_F32 || dt == FR_B200_T_BF16; }
+inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack { T v[V]; };
+// V elements, `n` of them there; whole: one access of V * sizeof(T) bytes
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T *p, int n, bool whole) {
+  if (whole) return *reinterpret_cast<const Pack<T, V> *>(p);
+  Pack<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : from_f<T>(0.f);
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n, bool whole) {
+  if (whole) { *reinterpret_cast<Pack<T, V> *>(p) = r; return; }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) p[i] = r.v[i];
+}
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+
+// log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in [0, 1].  log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3, by the odd series up
+// to s^15 (the first term left out is 3e-9 of the sum): time steps are 0.001 to 0.1, so that the small values need their relative
+// precision, which the logarithm of the rounded 1 + e has lost.  Relative error some 4e-7, most of it exp's.  NaN stays NaN.
+__device__ __forceinline__ float softplus(float v) {
+  const float e = ex2(-fabsf(v) * LOG2E), s = __fdividef(e, 2.f + e), q = s * s;
+  float p = 2.f / 15.f;
+  p = fmaf(p, q, 2.f / 13.f);
+  p = fmaf(p, q, 2.f / 11.f);
+  p = fmaf(p, q, 2.f / 9.f);
+  p = fmaf(p, q, 2.f / 7.f);
+  p = fmaf(p, q, 2.f / 5.f);
+  p = fmaf(p, q, 2.f / 3.f);
+  p = fmaf(p, q, 2.f);
+  return (v > 0.f ? v : 0.f) + s * p;
+}
+// v / (1 + exp(-v)); below -88 the divisor is infinite and the result -0, as the division's
+__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + ex2(-v * LOG2E)); }
+
+// ---- arguments ----
+// a [rows, width] piece of rows `ld` bytes apart
+struct Rows {
+  const void *p;
+  int64_t ld;      // bytes
+  int64_t width;   // bytes
+  int64_t rows;
+  uintptr_t first() const { return reinterpret_cast<uintptr_t>(p); }
+  uintptr_t end() const { return first() + (uintptr_t)((rows - 1) * ld + width); }
+};
+// Whether two pieces can have a byte in common: columns of the same rows do not.
+inline bool overlap(const Rows &a, const Rows &b) {
+  if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
+  if (a.end() <= b.first() || b.end() <= a.first()) return false;
+  if (a.ld != b.ld || a.ld <= 0) return true;
+  const int64_t d = (int64_t)((b.first() % (uintptr_t)a.ld + (uintptr_t)a.ld - a.first() % (uintptr_t)a.ld) % (uintptr_t)a.ld);
+  return !(d >= a.width && d + b.width <= a.ld);
+}
+
+// from / to of n streams over a pool of n_slots: nullptr: stream i has slot i.  -1: begins from zero / is not kept.  A slot is written by
+// one stream at most, and read by no other stream then: streams run side by side.
+int check_slots(int n, const void *state, int n_slots, const int32_t *from, const int32_t *to);
+
+// moves between slots of a pool: distinct destinations (see fr_b200_slots_copy)
+int check_moves(int n_slots, int n, const int32_t *src, const int32_t *dst);
+// what cleared slots hold besides zeros: `layers` vectors of n floats
+struct SlotFill { size_t offset, layer_stride; int layers, n; float value; };
+cudaError_t launch_slots_copy(void *pool, size_t bytes, size_t stride, int n_slots, int n, const int32_t *src, const int32_t *dst,
+                              const SlotFill *fill, cudaStream_t st);
+
+// Sequences of one launch, by value: a captured graph holds them, as it holds the ids of a decode step.
+constexpr int SEQ_CAP = 256;
+struct SeqTable {
+  int n;
+  int from[SEQ_CAP], to[SEQ_CAP];   // slots, or -1
+  long long first[SEQ_CAP + 1];     // rows first[i] .. first[i + 1] - 1 are sequence i
+};
+// Pieces of 2^shift rows: sequence i has the numbers from seq_key(i) on, at least one and as many as it has pieces; numbers behind
+// them, up to the next sequence's first, are of nobody.  (floor((a + b) / len) + 1 >= floor(a / len) + max(1, ceil(b / len)).)
+__host__ __device__ inline int seq_key(const SeqTable &t, int i, int shift) { return (int)((t.first[i] - t.first[0]) >> shift) + i; }
+inline int seq_items(const SeqTable &t, int shift) { return (int)((t.first[t.n] - t.first[0]) >> shift) + t.n; }
+__device__ inline int seq_of(const SeqTable &t, int item, int shift) {
+  int lo = 0, hi = t.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (seq_key(t, mid, shift) <= item) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+constexpr int SLOT_CAP = 512;
+struct SlotTable { int n, base; int from[SLOT_CAP], to[SLOT_CAP]; };   // streams base .. base + n - 1
+
+}  // namespace frb

@@ -8,18 +8,16 @@
 
 #include "../../include/fr_b200.h"
 #include "internal.h"
+#include "operators.cuh"
 
 using namespace frb;
 
 namespace {
-
 thread_local std::string g_op_err;
-int op_fail(int code, const std::string &msg) { g_op_err = msg; return code; }
-#define OP_CU(call)                                                                                          \
-  do {                                                                                                       \
-    cudaError_t e_ = (call);                                                                                 \
-    if (e_ != cudaSuccess) return op_fail(FR_B200_E_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
-  } while (0)
+}
+int frb::op_fail(int code, const std::string &msg) { g_op_err = msg; return code; }
+
+namespace {
 
 __device__ __forceinline__ float ldv(const void *p, size_t i, int dt) {
   return dt == FR_B200_T_F16 ? __half2float(reinterpret_cast<const __half *>(p)[i]) : reinterpret_cast<const float *>(p)[i];

@@ -40,8 +40,17 @@ enum {
 
 /* weight formats = the reference's strategy dtype strings (model.cpp:44-60) */
 enum { FR_B200_W_FP16 = 0, FR_B200_W_INT8 = 1, FR_B200_W_INT4 = 2 };
-/* tensor element types accepted by fr_b200_set_tensor (tensor.h:33-41) */
-enum { FR_B200_T_F16 = 0, FR_B200_T_F32 = 1 };
+/* tensor element types accepted by fr_b200_set_tensor (tensor.h:33-41); bf16 by the operators that say so */
+enum { FR_B200_T_F16 = 0, FR_B200_T_F32 = 1, FR_B200_T_BF16 = 2 };
+/* what fr_b200_linear and the convolution do to their sums */
+enum {
+  FR_B200_ACT_NONE = 0,
+  FR_B200_ACT_RELU2 = 1,     /* max(v, 0)^2 */
+  FR_B200_ACT_SILU = 2,      /* v / (1 + exp(-v)) */
+  FR_B200_ACT_SIGMOID = 3,
+  FR_B200_ACT_GELU = 4,      /* v (1 + erf(v / sqrt 2)) / 2 */
+  FR_B200_ACT_SOFTPLUS = 5   /* log(1 + exp(v)) */
+};
 /* model versions = the `.fr` "version" string (kernels/default/init_model.cpp:58-73) */
 enum { FR_B200_V4 = 4, FR_B200_V5_0 = 50, FR_B200_V5_1 = 51, FR_B200_V5_2 = 52 };
 
@@ -259,6 +268,67 @@ int fr_b200_elementwise(int op, const void *x, int x_dtype, const void *y, int y
 int fr_b200_matmul(const void *a, int a_dtype, int M, int K, const void *w, int w_dtype, int N, void *out, int out_dtype,
                    int device, void *stream);
 const char *fr_b200_op_last_error(void);
+
+/* ---- operators of a recurrent layer over DEVICE tensors as they lie ------------------------------------------------
+ * Projections with their epilogue, the short causal convolution, the selective state space scan, and the slots that hold
+ * the streams' states (the reference has none of them; they stand beside its recurrences above).  Common to all:
+ *   - tensors are [rows, width] pieces whose rows lie `ld` elements apart; dtype FR_B200_T_F16, _BF16 or _F32; parameters
+ *     (bias, weights of the convolution, A, D, dt_bias) are fp32.  Sums, states and statistics are fp32, each output is
+ *     rounded once.  No alignment beyond the element's is asked; rows and pointers of whole 16 bytes are faster;
+ *   - asynchronous on `stream`, on `device` whatever device is current (the caller's stays current); nothing is allocated,
+ *     nothing is synchronised, no result depends on the order of atomics: calls may be captured, and captured calls hold
+ *     the host arrays (sequences, slots) by value;
+ *   - host arrays are checked: FR_B200_E_ARG, with the reason in fr_b200_op_last_error(), and nothing is launched.
+ *     Outputs may not overlap inputs or the pool, except where it says so;
+ *   - sequences: `starts` (host [n_seq + 1], not decreasing, within 0 .. rows) gives sequence i the rows starts[i] ..
+ *     starts[i + 1] - 1, none allowed; NULL: one sequence of all rows.  Rows of no sequence stay as they were in `out`;
+ *   - slots: the state of stream i is read from slot from[i] of the pool `state` (slots state_stride elements apart) and
+ *     its state after the last row written to slot to[i] (host arrays; NULL: slot i).  -1: begins from zero / is not kept.
+ *     A slot is written by one stream of a call at most, and then read by no other.  state NULL: all from zero, none kept.
+ *     An empty sequence hands its state on. */
+
+/* out[rows, N] = residual + act(x[rows, K] . w[N, K]^T + bias[N]); bias and residual may be NULL.  x, w: f16 or bf16 (the
+ * same); out and residual: the type of x, or f32.  residual may be out itself.  Operands multiply on the tensor cores with
+ * fp32 sums whose order depends on the shape alone; up to 4,194,304 rows. */
+int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, int64_t rows, int K, int N, const float *bias, int act,
+                   const void *residual, int64_t ldr, void *out, int64_t ldo, int out_dtype, int device, void *stream);
+
+/* y[t, d] = act(bias[d] + sum_j w[d, j] x[t - (taps - 1) + j, d]), act none or silu, taps 2 to 4; w [D, taps], bias [D] or NULL.
+ * A state is the last taps - 1 rows, [taps - 1, D] in the type of x, oldest first: they come before a sequence's first row. */
+int fr_b200_conv_seq(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const float *w, int taps, const float *bias, int act,
+                     const int32_t *starts, int n_seq, void *state, int64_t state_stride, int n_slots, const int32_t *from, const int32_t *to,
+                     void *out, int64_t ldo, int device, void *stream);
+/* The same for one row of each of n streams (row i: stream i). */
+int fr_b200_conv_step(const void *x, int64_t ldx, int dtype, int n, int D, const float *w, int taps, const float *bias, int act, void *state,
+                      int64_t state_stride, int n_slots, const int32_t *from, const int32_t *to, void *out, int64_t ldo, int device, void *stream);
+
+/* For every channel d, its N states (1 to 128) and the rows of a sequence in order:
+ *   delta = softplus(dt + dt_bias)  (dt_softplus 0: dt + dt_bias)
+ *   h[n] <- exp(delta A[d, n]) h[n] + delta x B[g, n]
+ *   out = (sum_n C[g, n] h[n] + Dskip[d] x) * silu(z)
+ * x, dt, z, out: [rows, D]; B, C: [rows, groups * N], channel d of group g = d / (D / groups); A: [D, N]; Dskip, dt_bias [D]
+ * or NULL (0), z NULL: no gate.  A state is [D, N] fp32.  work: fr_b200_ssm_seq_workspace() bytes of device memory that
+ * the call has to itself until its work on the stream is done (0 for most shapes). */
+size_t fr_b200_ssm_seq_workspace(int64_t rows, int n_seq, int D, int N);
+int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, const float *A, const void *B, int64_t ldb, const void *C,
+                    int64_t ldc, const float *Dskip, const void *z, int64_t ldz, const float *dt_bias, int dt_softplus, int dtype, int64_t rows,
+                    int D, int N, int groups, const int32_t *starts, int n_seq, float *state, int64_t state_stride, int n_slots,
+                    const int32_t *from, const int32_t *to, void *out, int64_t ldo, void *work, size_t work_bytes, int device, void *stream);
+/* The same for one row of each of n streams. */
+int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, const float *A, const void *B, int64_t ldb, const void *C,
+                     int64_t ldc, const float *Dskip, const void *z, int64_t ldz, const float *dt_bias, int dt_softplus, int dtype, int n, int D,
+                     int N, int groups, float *state, int64_t state_stride, int n_slots, const int32_t *from, const int32_t *to, void *out,
+                     int64_t ldo, int device, void *stream);
+
+/* Slots of a pool copied, forked, moved or cleared: slot dst[i] becomes what slot src[i] was before the call, src -1: zeros.
+ * Slots are slot_bytes long and slot_stride bytes apart; up to 65535 slots, up to 4096 moves, every dst once.  What lies
+ * between slots stays as it was. */
+int fr_b200_slots_copy(void *pool, size_t slot_bytes, size_t slot_stride, int n_slots, int n, const int32_t *src, const int32_t *dst, int device,
+                       void *stream);
+/* The same for the state slots of a model (fork a prompt's state into several streams, close the gaps that finished streams leave); src -1:
+ * the initial state of fr_b200_state_reset.  Ordered on `stream` like the model's other calls; not on a capturing stream (FR_B200_E_STATE). */
+int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_t *dst, void *stream);
+
 
 /* out[M,N] = epilogue(A[M,K] @ W[K,N]) on the tcgen05 tensor cores, fp16 operands, fp32 accumulate: the seq-mode
  * replacement of gemm_cublas_tensor (kernels/cuda/matmul.cpp:105-122) with the element-wise kernels that follow
