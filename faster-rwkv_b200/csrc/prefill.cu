@@ -17,6 +17,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
 
 namespace frb {
 
@@ -86,78 +87,9 @@ constexpr int G_THREADS = 192;
 constexpr uint32_t G_A_BYTES = GBM * GBK * 2;
 constexpr int ST_GEMM_TIMEOUT = 201;
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-               : "memory");
-}
-// shared-memory matrix descriptor of a K-major tile whose rows are 128 bytes (64 halfs), 128-byte swizzle, eight-row
-// groups 1024 bytes apart: start address / 16 in bits 0-13, leading offset (unused for swizzled K-major) = 1 in
-// bits 16-29, stride offset 1024 / 16 in bits 32-45, descriptor version 1 in bits 46-47, layout 2 (128B) in bits 61-63
-__device__ __forceinline__ uint64_t umma_desc_k128(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr & 0x3ffffu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
 // instruction descriptor, kind::f16: D = f32 (bits 4-5 = 1), A = B = f16 (0), both K-major (0), N / 8 in bits 17-22,
 // M / 16 in bits 24-28
 // (built per tile width inside the kernel)
-
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// the tensor maps are launch parameters: their first use would be a cold fetch in front of the first tile
-__device__ __forceinline__ void prefetch_tmap(const CUtensorMap *m) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-}
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// One lane of a converged warp, the same one every time.  The warps that issue MMAs and copies run their loops whole and elect a lane for the
-// instruction: inside a branch that one lane took alone, descriptors and addresses move to uniform registers one by one and an MMA took
-// about 100 clocks to issue (a slice of int8 over 160 columns 0.34 us, now 0.24; of int4 0.56, now 0.38).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
-  return one != 0;
-}
-
-// Place in a ring of barriers.  Its slot and phase are counted: a division by a depth that only the launch knows costs 100
-// to 200 clocks of a chain that takes 300 to 1,000 per slice, and every role had two to four of them.
-struct Ring {
-  int slot = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next(int depth) {
-    if (++slot == depth) { slot = 0; phase ^= 1u; }
-  }
-};
 
 // By the fast exponential (2 + 1.17 |v| ulp by CUDA's bounds) and division (2 ulp): a relative error of up to 5e-7 for v > 0 and 1.7e-6 at
 // v = -8, where the value is 3e-4.  The fp16 rounding of a single result (4.9e-4) hides it; where the low half is stored as well (streams, short
@@ -320,40 +252,6 @@ __device__ __forceinline__ void tile_out_end() {
   if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// the address, in the cluster's shared window, of this CTA's shared address `a` in CTA `rank`
-__device__ __forceinline__ uint32_t mapa_u32(uint32_t a, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// tile into this CTA's shared memory, bytes counted on a barrier of either CTA of the pair
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
-      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Arrive on a barrier of either CTA of the cluster (address from mapa_u32).  Relaxed: it hands over no memory, but columns of TMEM, whose
-// writes are complete (tcgen05.wait::st) and ordered by the tcgen05 fences on both sides.  With .release it took 500 to 900 clocks, a slice of
-// int8 0.70 us instead of 0.50.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
 // ---- TMEM of a pair of CTAs ----
 // tcgen05.alloc / dealloc with cta_group::2 are one operation of a warp of each CTA, and ask that the other CTA has been launched and has not
 // left: they stand between cluster barriers.  An SM lets one CTA at a time allocate, from its allocation until it gives the permit back, so two
@@ -452,13 +350,6 @@ __device__ __forceinline__ void pair_tmem_end(const PairTmem *t, int warp, uint3
   __syncwarp();
   cluster_sync();
 }
-// arrives on the barrier at this offset in both CTAs of the pair
-__device__ __forceinline__ void umma_commit_pair(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(smem_u32(bar)), "h"((uint16_t)3)
-               : "memory");
-}
-
 // ------------------------------------------------------------------------------------------------
 // fp16 weights, more than 128 rows (64, with low halves): out^T[256 channels, BN rows] per pair of CTAs (BN a multiple of 32 up to 256,
 // chosen at launch).  The pair is one tcgen05.mma.cta_group::2: each CTA holds the weights of its own 128 channels and
@@ -1142,29 +1033,6 @@ __global__ void __launch_bounds__(256) gemm_finish_kernel(const __grid_constant_
   }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
-
-bool encode_map(CUtensorMap *map, CUtensorMapDataType type, int rank, void *base, const cuuint64_t *dims, const cuuint64_t *strides,
-                const cuuint32_t *box, bool swizzle, bool promote) {
-  EncodeTiledFn fn = encode_fn();
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return fn && fn(map, type, (cuuint32_t)rank, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                  promote ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 static_assert(sizeof(CUtensorMap) == sizeof(TensorMapBytes), "tensor maps are kept as bytes");
 // An activation's map out of the forward pass's cache, or encoded.  (A map takes about 0.2 us, a launch of few rows needs up to 15.)
 template <typename Encode>
