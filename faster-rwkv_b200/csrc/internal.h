@@ -201,6 +201,7 @@ constexpr int GEMM_GROUP_MAX = 4;
 constexpr int GEMM_SMALL_M = 1024;    // up to this many rows the GEMM puts the weights along the MMA rows (and splits K, given scratch)
 constexpr int GEMM_SPLIT_MAX = 16;
 int device_sm_count();   // SMs of the current device
+bool pdl_enabled();      // kernels are launched ahead of the end of the ones before them (FR_B200_PDL, on unless 0)
 cudaError_t launch_gemm_f16(const GemmArgs &g, cudaStream_t st);   // one GEMM
 // n <= 4 GEMMs with equal M in one launch, after gemm_prepare() for the device
 cudaError_t launch_gemm_group(const GemmArgs *probs, int n, cudaStream_t st, int *defer_split = nullptr);

@@ -14,6 +14,8 @@
 #include <vector>
 
 #include "../../include/fr_b200.h"
+#include "common.cuh"
+#include "internal.h"
 
 namespace frb {
 
@@ -105,6 +107,31 @@ __device__ __forceinline__ float softplus(float v) {
 }
 // v / (1 + exp(-v)); below -88 the divisor is infinite and the result -0, as the division's
 __device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + ex2(-v * LOG2E)); }
+
+// ---- launches ----
+// As the row kernels': the kernel may become resident, and set itself up, while the one before it in the stream drains.  Every thread calls
+// pdl_wait() before it touches global memory (a kernel none of whose threads waited could end before the one before it), and
+// pdl_trigger() as soon as the CTA holds all it needs (its tensor memory), so that none behind can keep it from that.
+template <typename... KArgs, typename... Args>
+cudaError_t op_launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, Args &&...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)cluster; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
 
 // ---- arguments ----
 // a [rows, width] piece of rows `ld` bytes apart

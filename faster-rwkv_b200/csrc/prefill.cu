@@ -36,16 +36,17 @@ int device_sm_count() {
 
 thread_local long long row_launches = 0;
 
+bool pdl_enabled() {
+  static const int on = [] { const char *v = getenv("FR_B200_PDL"); return !(v && v[0] == '0'); }();
+  return on != 0;
+}
+
 namespace {
 
 // Every kernel of the seq / batch chain goes through here.  With FR_B200_PDL != 0 (the default) the launch carries
 // the programmatic stream-serialisation attribute: the kernel's CTAs may be scheduled, and run their set-up, while the
 // kernel before it in the stream drains; each kernel calls pdl_wait() before it touches global memory, so the data
 // dependences are those of plain stream order.
-bool pdl_enabled() {
-  static const int on = [] { const char *v = getenv("FR_B200_PDL"); return !(v && v[0] == '0'); }();
-  return on != 0;
-}
 template <typename... KArgs, typename... Args>
 cudaError_t launch_cluster_k(void (*kern)(KArgs...), int cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
   cudaLaunchConfig_t cfg;

@@ -114,6 +114,19 @@ def test_linear_pieces_of_wider_rows(pkg, rows, k, n, shift):
     assert torch.equal(O, keep)
 
 
+@pytest.mark.parametrize("rows,k,n", [(5, 64, 70), (40, 640, 333), (100, 4096, 130), (260, 512, 77), (700, 256, 700)])
+@pytest.mark.parametrize("out_dtype", [F16, F32])
+def test_linear_with_ragged_results(pkg, rows, k, n, out_dtype):
+    """operands at 16-byte boundaries, residual and out off them"""
+    x, w, b = _rand(rows, k, dtype=F16), _rand(n, k, dtype=F16, scale=k ** -0.5, seed=1), _rand(n, seed=2)
+    R, O = _rand(rows, n + 5, dtype=out_dtype, seed=3), torch.full((rows, n + 3), 9.0, dtype=out_dtype, device="cuda")
+    for act, res in (("gelu", R[:, 2:2 + n]), ("none", None)):
+        pkg.linear(x, w, b, activation=act, residual=res, out=O[:, 1:1 + n])
+        want, err = _linear_want(x, w, b, act, res)
+        _check(O[:, 1:1 + n], want, err, act)
+        assert bool((O[:, 0] == 9).all()) and bool((O[:, n + 1:] == 9).all())
+
+
 @pytest.mark.parametrize("rows", [1, 20, 200, 500])
 def test_linear_onto_the_residual(pkg, rows):
     x, w = _rand(rows, 320, dtype=F16), _rand(264, 320, dtype=F16, scale=0.1, seed=1)
