@@ -11,6 +11,23 @@ using namespace frb;
 
 namespace {
 
+// V elements, n of them there, as one access where that may be (`whole`): of epilogues and last pieces
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_some(const T *p, int n, bool whole) {
+  if (whole) return *reinterpret_cast<const Pack<T, V> *>(p);
+  Pack<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : from_f<T>(0.f);
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_some(T *p, const Pack<T, V> &r, int n, bool whole) {
+  if (whole) { *reinterpret_cast<Pack<T, V> *>(p) = r; return; }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) p[i] = r.v[i];
+}
+
 struct LinearArgs {
   const void *x, *w, *residual;
   const float *bias;
@@ -192,9 +209,9 @@ __global__ void __launch_bounds__(32 * NW, CTAS) linear_rows_kernel(const Linear
     Frag w[2], x[NT];
     const int n = a.K - k0 - t * 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w[i].p = load_pack<T, 8>(wp[i] + k0, n, n >= 8);
+    for (int i = 0; i < 2; ++i) w[i].p = load_some<T, 8>(wp[i] + k0, n, n >= 8);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j].p = load_pack<T, 8>(xp[j] + k0, n, n >= 8);
+    for (int j = 0; j < NT; ++j) x[j].p = load_some<T, 8>(xp[j] + k0, n, n >= 8);
     multiply(w, x);
   }
   pdl_trigger();   // (not earlier: CTAs of the next kernel would crowd on the SMs that have few of this one's)
@@ -225,7 +242,7 @@ struct Finish {
   using O = typename std::conditional<OUT32, float, T>::type;
   Pack<O, V> res[RES ? R : 1];
   __device__ __forceinline__ void ask(const LinearArgs &a, int i, long long m, int n, bool whole) {
-    if (RES) res[RES ? i : 0] = load_pack<O, V>(reinterpret_cast<const O *>(a.residual) + m * a.ldr + n, a.N - n, whole);
+    if (RES) res[RES ? i : 0] = load_some<O, V>(reinterpret_cast<const O *>(a.residual) + m * a.ldr + n, a.N - n, whole);
   }
   __device__ __forceinline__ void act(const LinearArgs &a, float (&v)[R * V], const float (&bias)[V]) {
 #pragma unroll
@@ -236,7 +253,7 @@ struct Finish {
     Pack<O, V> o;
 #pragma unroll
     for (int k = 0; k < V; ++k) o.v[k] = from_f<O>(RES ? v[k] + to_f(res[RES ? i : 0].v[k]) : v[k]);
-    store_pack<O, V>(reinterpret_cast<O *>(a.out) + m * a.ldo + n, o, a.N - n, whole);
+    store_some<O, V>(reinterpret_cast<O *>(a.out) + m * a.ldo + n, o, a.N - n, whole);
   }
 };
 
@@ -521,7 +538,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
         if (RES && whole)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (row0 + 8 * r < a.M) res[RES ? r : 0] = load_pack<O, 8>(reinterpret_cast<const O *>(a.residual) + (row0 + 8 * r) * a.ldr + n, 8, true);
+            if (row0 + 8 * r < a.M) res[RES ? r : 0] = load_some<O, 8>(reinterpret_cast<const O *>(a.residual) + (row0 + 8 * r) * a.ldr + n, 8, true);
         const float bias = a.bias && n0 + c0 + lane < a.N ? a.bias[n0 + c0 + lane] : 0.f;
         tmem_wait(acc);
         float v[32];
@@ -569,7 +586,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
 #pragma unroll
               for (int k = 0; k < 8; ++k) o.v[k] = from_f<O>(RES ? s[k] + to_f(res[RES ? r : 0].v[k]) : s[k]);
             }
-            if (row0 + 8 * r < a.M) store_pack<O, 8>(out + 8ll * r * a.ldo, o, 8, true);
+            if (row0 + 8 * r < a.M) store_some<O, 8>(out + 8ll * r * a.ldo, o, 8, true);
           }
         } else {   // columns that end inside, or rows that are not whole 16 bytes apart: a channel per lane
 #pragma unroll
@@ -610,15 +627,6 @@ bool rows_map(CUtensorMap *map, const void *base, long long rows, int K, long lo
   const cuuint32_t box[2] = {(cuuint32_t)LK, (cuuint32_t)box_rows};
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, true, true);
 }
-template <typename K>
-cudaError_t allow_smem(K kern, uint64_t &told) {   // once per device
-  int dev;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (dev < 64 && (told >> dev & 1))) return e;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-  if (e == cudaSuccess && dev < 64) told |= 1ull << dev;
-  return e;
-}
 template <typename T, int NT, int NW, int CTAS>
 cudaError_t rows_launch(const LinearArgs &a, cudaStream_t st) {
   return op_launch(linear_rows_kernel<T, NT, NW, CTAS>, dim3((a.N + 15) / 16), 32 * NW, 0, st, 1, a);
@@ -634,7 +642,7 @@ cudaError_t tile_launch(const LinearArgs &a, int bn, int split, cudaStream_t st)
   const int kind = a.out_f32 * 2 + (a.residual != nullptr);
   const auto kern = kind == 0 ? linear_tile_kernel<T, false, false> : kind == 1 ? linear_tile_kernel<T, false, true>
                   : kind == 2 ? linear_tile_kernel<T, true, false> : linear_tile_kernel<T, true, true>;
-  cudaError_t e = allow_smem(kern, told[kind]);
+  cudaError_t e = allow_smem(kern, 227 * 1024, told[kind]);
   if (e != cudaSuccess) return e;
   LinearPlan p;
   LinearMaps maps;
@@ -658,7 +666,7 @@ cudaError_t pair_launch(const LinearArgs &a, int bn, cudaStream_t st) {
   const int kind = a.out_f32 * 2 + (a.residual != nullptr);
   const auto kern = kind == 0 ? linear_pair_kernel<T, false, false> : kind == 1 ? linear_pair_kernel<T, false, true>
                   : kind == 2 ? linear_pair_kernel<T, true, false> : linear_pair_kernel<T, true, true>;
-  cudaError_t e = allow_smem(kern, told[kind]);
+  cudaError_t e = allow_smem(kern, 227 * 1024, told[kind]);
   if (e != cudaSuccess) return e;
   LinearPlan p;
   LinearMaps maps;

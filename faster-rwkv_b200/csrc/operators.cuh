@@ -66,21 +66,25 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack { T v[V]; };
-// V elements, `n` of them there; whole: one access of V * sizeof(T) bytes
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T *p, int n, bool whole) {
-  if (whole) return *reinterpret_cast<const Pack<T, V> *>(p);
+// V elements from p on, of which `n` are there (at least one; the others repeat the last).  VEC: one access, all are there; else one by one.  A kernel is
+// compiled for either: where two ways of loading meet, the load is waited for, and nothing is in flight behind it any more (a convolution
+// of 4001 x 5120 took 54 us that way, 17 with one).
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ Pack<T, V> load_pack(const T *p, int n) {
   Pack<T, V> r;
+  if constexpr (VEC) r = *reinterpret_cast<const Pack<T, V> *>(p);
+  else
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : from_f<T>(0.f);
+    for (int i = 0; i < V; ++i) r.v[i] = p[i < n ? i : n - 1];
   return r;
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n, bool whole) {
-  if (whole) { *reinterpret_cast<Pack<T, V> *>(p) = r; return; }
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n) {
+  if constexpr (VEC) *reinterpret_cast<Pack<T, V> *>(p) = r;
+  else
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (i < n) p[i] = r.v[i];
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = r.v[i];
 }
 
 __device__ __forceinline__ float ex2(float v) {
@@ -131,6 +135,17 @@ cudaError_t op_launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t sme
   cfg.attrs = at;
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// more shared memory than 48 KB: once per kernel and device
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, uint64_t &told) {
+  int dev;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (told >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) told |= 1ull << dev;
+  return e;
 }
 
 // ---- arguments ----

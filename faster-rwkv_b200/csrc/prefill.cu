@@ -1706,24 +1706,6 @@ constexpr int WKV_THREADS = 64;
 // Packed fp32 pairs (fma.rn.f32x2 / mul.rn.f32x2: two fp32 operations per instruction on sm_100).  The scan is bound
 // by the issue rate of its multiply-adds, so the state is kept as pairs over neighbouring key rows: k, r and the decay
 // then come out of shared memory already paired, and only v needs a broadcast pair per token.
-__device__ __forceinline__ unsigned long long pack_f2(float lo, float hi) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack_f2(unsigned long long v, float &lo, float &hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ unsigned long long fma_f2(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ unsigned long long mul_f2(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 // y_t[j] = sum_i r_i (u_i k_i v_j + s_ij) = v_j (sum_i r_i u_i k_i) + sum_i r_i s_ij;  s_ij <- w_i s_ij + k_i v_j.
 // Thread (jg, iq) owns key rows iq*16 .. +15 of value columns jg + 16 q (q = 0..3): 32 pairs.

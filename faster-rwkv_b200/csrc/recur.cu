@@ -5,6 +5,7 @@
 
 #include "internal.h"
 #include "operators.cuh"
+#include "ssm.cuh"
 
 using namespace frb;
 
@@ -76,41 +77,53 @@ struct ConvArgs {
 };
 constexpr int CONV_SHIFT = 4, CONV_ROWS = 1 << CONV_SHIFT;   // rows of a piece; at least W - 1, so that only a sequence's first piece meets its state
 
-template <int W, int V>
+template <int W, int V, bool VEC>
 struct ConvTaps {
-  float w[V][W], b[V];
+  float w[V * W], b[V];
   __device__ __forceinline__ void load(const ConvArgs &a, int c, int n) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      b[i] = i < n && a.bias ? a.bias[c + i] : 0.f;
+    for (int i = 0; i < V * W; i += 4) {
+      const Pack<float, 4> v = load_pack<float, 4, VEC>(a.w + (size_t)c * W + i, max(n * W - i, 1));
 #pragma unroll
-      for (int j = 0; j < W; ++j) w[i][j] = i < n ? a.w[(size_t)(c + i) * W + j] : 0.f;
+      for (int q = 0; q < 4; ++q) w[i + q] = v.v[q];
     }
+    const Pack<float, 4> v = load_pack<float, 4, VEC>(a.bias ? a.bias + c : a.w, n);   // (no bias: something that is there, and not taken)
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = a.bias ? v.v[i] : 0.f;
   }
 };
 
-template <typename T, int W, int V>
-__global__ void __launch_bounds__(128) conv_seq_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab, int vec) {
+// CONV_ROWS rows of 4 channels a thread, all asked for at once, the window in registers
+template <typename T, int W, bool VEC>
+__global__ void __launch_bounds__(128) conv_seq_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
+  constexpr int V = 4;
   const int c = (blockIdx.y * 128 + threadIdx.x) * V;
-  if (c >= a.D) return;
   const int item = blockIdx.x, s = seq_of(tab, item, CONV_SHIFT), piece = item - seq_key(tab, s, CONV_SHIFT);
   const long long first = tab.first[s], end = tab.first[s + 1], row0 = first + (long long)piece * CONV_ROWS;
-  if (piece > 0 && row0 >= end) return;
-  const int n = a.D - c < V ? a.D - c : V;
-  const bool whole = V > 1 && vec && n == V;
-  const T *x = reinterpret_cast<const T *>(a.x) + c;
-  T *out = reinterpret_cast<T *>(a.out) + c, *state = reinterpret_cast<T *>(a.state) + c;
-  ConvTaps<W, V> taps;
+  pdl_wait();
+  pdl_trigger();
+  if (c >= a.D || (piece > 0 && row0 >= end)) return;
+  const int n = a.D - c < V ? a.D - c : V, rows = end - row0 < CONV_ROWS ? (int)(end - row0) : CONV_ROWS;
+  const T *x = reinterpret_cast<const T *>(a.x) + c, *xr = x + row0 * a.ldx;
+  T *out = reinterpret_cast<T *>(a.out) + c + row0 * a.ldo, *state = reinterpret_cast<T *>(a.state) + c;
+  const int from = piece == 0 ? tab.from[s] : 0;
+  // what lies before the piece: rows of x, or of the state, or zeros
+  const T *back = piece > 0 ? xr - (W - 1) * a.ldx : state + (long long)max(from, 0) * a.state_stride;
+  const long long back_ld = piece > 0 ? a.ldx : a.D;
+  const bool zeros = piece == 0 && from < 0;
+  Pack<T, V> before[W - 1], in[CONV_ROWS];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+    for (int i = 0; i < V; ++i) before[j].v[i] = from_f<T>(0.f);
+  if (!zeros)
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) before[j] = load_pack<T, V, VEC>(back + j * back_ld, n);
+  if (rows > 0)
+#pragma unroll
+    for (int r = 0; r < CONV_ROWS; ++r) in[r] = load_pack<T, V, VEC>(xr + (long long)min(r, rows - 1) * a.ldx, n);
+  ConvTaps<W, V, VEC> taps;
   taps.load(a, c, n);
-  Pack<T, V> before[W - 1];
-#pragma unroll
-  for (int j = 0; j < W - 1; ++j) {
-    if (piece > 0) before[j] = load_pack<T, V>(x + (row0 - (W - 1) + j) * a.ldx, n, whole);
-    else if (tab.from[s] >= 0) before[j] = load_pack<T, V>(state + tab.from[s] * a.state_stride + (long long)j * a.D, n, whole);
-    else
-#pragma unroll
-      for (int i = 0; i < V; ++i) before[j].v[i] = from_f<T>(0.f);
-  }
   if (piece == 0 && tab.to[s] >= 0) {
     // the last W - 1 of (state, rows).  No other CTA looks at either slot, and x does not change.
     const long long len = end - first;
@@ -118,15 +131,12 @@ __global__ void __launch_bounds__(128) conv_seq_kernel(const ConvArgs a, const _
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
       const long long at = len - (W - 1) + j;
-      Pack<T, V> v;
-      if (at >= 0) v = load_pack<T, V>(x + (first + at) * a.ldx, n, whole);
-      else {
-        v = before[0];
+      Pack<T, V> v = before[0];
 #pragma unroll
-        for (int q = 1; q < W - 1; ++q)
-          if (q == (int)(W - 1 + at)) v = before[q];
-      }
-      store_pack<T, V>(to + (long long)j * a.D, v, n, whole);
+      for (int q = 1; q < W - 1; ++q)
+        if (q == (int)(W - 1 + at)) v = before[q];
+      if (at >= 0) v = load_pack<T, V, VEC>(x + (first + at) * a.ldx, n);
+      store_pack<T, V, VEC>(to + (long long)j * a.D, v, n);
     }
   }
   float win[W - 1][V];
@@ -134,98 +144,82 @@ __global__ void __launch_bounds__(128) conv_seq_kernel(const ConvArgs a, const _
   for (int j = 0; j < W - 1; ++j)
 #pragma unroll
     for (int i = 0; i < V; ++i) win[j][i] = to_f(before[j].v[i]);
-  const int rows = end - row0 < CONV_ROWS ? (int)(end - row0) : CONV_ROWS;
-  constexpr int AHEAD = 8;
 #pragma unroll
-  for (int g = 0; g < CONV_ROWS; g += AHEAD) {
-    if (g >= rows) break;
-    Pack<T, V> in[AHEAD];
+  for (int r = 0; r < CONV_ROWS; ++r) {
+    if (r >= rows) break;
+    Pack<T, V> o;
 #pragma unroll
-    for (int r = 0; r < AHEAD; ++r)
-      if (g + r < rows) in[r] = load_pack<T, V>(x + (row0 + g + r) * a.ldx, n, whole);
+    for (int i = 0; i < V; ++i) {
+      const float v = to_f(in[r].v[i]);
+      float acc = taps.b[i];
 #pragma unroll
-    for (int r = 0; r < AHEAD; ++r) {
-      if (g + r >= rows) break;
-      Pack<T, V> o;
+      for (int j = 0; j < W - 1; ++j) acc = fmaf(taps.w[i * W + j], win[j][i], acc);
+      acc = fmaf(taps.w[i * W + W - 1], v, acc);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float v = to_f(in[r].v[i]);
-        float acc = taps.b[i];
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) acc = fmaf(taps.w[i][j], win[j][i], acc);
-        acc = fmaf(taps.w[i][W - 1], v, acc);
-#pragma unroll
-        for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-        win[W - 2][i] = v;
-        o.v[i] = from_f<T>(a.silu ? silu(acc) : acc);
-      }
-      store_pack<T, V>(out + (row0 + g + r) * a.ldo, o, n, whole);
+      for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
+      win[W - 2][i] = v;
+      o.v[i] = from_f<T>(a.silu ? silu(acc) : acc);
     }
+    store_pack<T, V, VEC>(out + (long long)r * a.ldo, o, n);
   }
 }
 
-template <typename T, int W, int V>
-__global__ void __launch_bounds__(128) conv_step_kernel(const ConvArgs a, const __grid_constant__ SlotTable tab, int vec) {
+template <typename T, int W, bool VEC>
+__global__ void __launch_bounds__(128) conv_step_kernel(const ConvArgs a, const __grid_constant__ SlotTable tab) {
+  constexpr int V = 4;
   const int c = (blockIdx.x * 128 + threadIdx.x) * V;
+  pdl_wait();
+  pdl_trigger();
   if (c >= a.D) return;
-  const int s = blockIdx.y, n = a.D - c < V ? a.D - c : V;
-  const bool whole = V > 1 && vec && n == V;
+  const int s = blockIdx.y, n = a.D - c < V ? a.D - c : V, from = tab.from[s];
   const long long row = tab.base + s;
   T *state = reinterpret_cast<T *>(a.state) + c;
   Pack<T, V> win[W];
-  win[W - 1] = load_pack<T, V>(reinterpret_cast<const T *>(a.x) + row * a.ldx + c, n, whole);
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) {
-    if (tab.from[s] >= 0) win[j] = load_pack<T, V>(state + tab.from[s] * a.state_stride + (long long)j * a.D, n, whole);
-    else
+  for (int j = 0; j < W - 1; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[j].v[i] = from_f<T>(0.f);
-  }
-  ConvTaps<W, V> taps;
+    for (int i = 0; i < V; ++i) win[j].v[i] = from_f<T>(0.f);
+  win[W - 1] = load_pack<T, V, VEC>(reinterpret_cast<const T *>(a.x) + row * a.ldx + c, n);
+  if (from >= 0)
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) win[j] = load_pack<T, V, VEC>(state + from * a.state_stride + (long long)j * a.D, n);
+  ConvTaps<W, V, VEC> taps;
   taps.load(a, c, n);
   Pack<T, V> o;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float acc = taps.b[i];
 #pragma unroll
-    for (int j = 0; j < W; ++j) acc = fmaf(taps.w[i][j], to_f(win[j].v[i]), acc);
+    for (int j = 0; j < W; ++j) acc = fmaf(taps.w[i * W + j], to_f(win[j].v[i]), acc);
     o.v[i] = from_f<T>(a.silu ? silu(acc) : acc);
   }
-  store_pack<T, V>(reinterpret_cast<T *>(a.out) + row * a.ldo + c, o, n, whole);
+  store_pack<T, V, VEC>(reinterpret_cast<T *>(a.out) + row * a.ldo + c, o, n);
   if (tab.to[s] >= 0)
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) store_pack<T, V>(state + tab.to[s] * a.state_stride + (long long)j * a.D, win[j + 1], n, whole);
+    for (int j = 0; j < W - 1; ++j) store_pack<T, V, VEC>(state + tab.to[s] * a.state_stride + (long long)j * a.D, win[j + 1], n);
 }
 
-template <typename T, int W, int V>
-cudaError_t conv_seq_launch(const ConvArgs &a, const SeqTable &t, int vec, cudaStream_t st) {
-  const dim3 grid(seq_items(t, CONV_SHIFT), (a.D + 128 * V - 1) / (128 * V));
-  conv_seq_kernel<T, W, V><<<grid, 128, 0, st>>>(a, t, vec);
-  return cudaGetLastError();
+template <typename T, int W, bool VEC>
+cudaError_t conv_go(const ConvArgs &a, const SeqTable &t, cudaStream_t st) {
+  return op_launch(conv_seq_kernel<T, W, VEC>, dim3(seq_items(t, CONV_SHIFT), (a.D + 511) / 512), 128, 0, st, 1, a, t);
 }
-template <typename T, int W, int V>
-cudaError_t conv_step_launch(const ConvArgs &a, const SlotTable &t, int vec, cudaStream_t st) {
-  const dim3 grid((a.D + 128 * V - 1) / (128 * V), t.n);
-  conv_step_kernel<T, W, V><<<grid, 128, 0, st>>>(a, t, vec);
-  return cudaGetLastError();
+template <typename T, int W, bool VEC>
+cudaError_t conv_go(const ConvArgs &a, const SlotTable &t, cudaStream_t st) {
+  return op_launch(conv_step_kernel<T, W, VEC>, dim3((a.D + 511) / 512, t.n), 128, 0, st, 1, a, t);
+}
+template <typename T, int W, typename TAB>
+cudaError_t conv_vec(const ConvArgs &a, const TAB &t, int vec, cudaStream_t st) {
+  return vec ? conv_go<T, W, true>(a, t, st) : conv_go<T, W, false>(a, t, st);
 }
 template <typename T, typename TAB>
-cudaError_t conv_launch(int taps, const ConvArgs &a, const TAB &t, int vec, cudaStream_t st) {
-  if constexpr (std::is_same<TAB, SeqTable>::value) {
-    if (taps == 2) return conv_seq_launch<T, 2, 4>(a, t, vec, st);
-    if (taps == 3) return conv_seq_launch<T, 3, 4>(a, t, vec, st);
-    return conv_seq_launch<T, 4, 4>(a, t, vec, st);
-  } else {
-    if (taps == 2) return conv_step_launch<T, 2, 4>(a, t, vec, st);
-    if (taps == 3) return conv_step_launch<T, 3, 4>(a, t, vec, st);
-    return conv_step_launch<T, 4, 4>(a, t, vec, st);
-  }
+cudaError_t conv_taps(int taps, const ConvArgs &a, const TAB &t, int vec, cudaStream_t st) {
+  return taps == 2 ? conv_vec<T, 2>(a, t, vec, st) : taps == 3 ? conv_vec<T, 3>(a, t, vec, st) : conv_vec<T, 4>(a, t, vec, st);
 }
 template <typename TAB>
 cudaError_t conv_any(int dt, int taps, const ConvArgs &a, const TAB &t, int vec, cudaStream_t st) {
-  if (dt == FR_B200_T_F16) return conv_launch<__half>(taps, a, t, vec, st);
-  if (dt == FR_B200_T_BF16) return conv_launch<__nv_bfloat16>(taps, a, t, vec, st);
-  return conv_launch<float>(taps, a, t, vec, st);
+  if (dt == FR_B200_T_F16) return conv_taps<__half>(taps, a, t, vec, st);
+  if (dt == FR_B200_T_BF16) return conv_taps<__nv_bfloat16>(taps, a, t, vec, st);
+  return conv_taps<float>(taps, a, t, vec, st);
 }
 
 // what both entries ask of their arguments; vec: rows and slots can be taken four elements at a time
@@ -247,304 +241,93 @@ int conv_check(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const
   OP_REQUIRE(!overlap(rx, rs) && !overlap(ro, rs), "the pool of states overlaps x or out");
   *a = {x, out, state, w, bias, ldx, ldo, state_stride, D, act == FR_B200_ACT_SILU};
   const size_t v = 4 * es;
-  *vec = aligned(x, v) && aligned(out, v) && aligned(state, v) && ldx % 4 == 0 && ldo % 4 == 0 && state_stride % 4 == 0 && D % 4 == 0;
+  *vec = aligned(x, v) && aligned(out, v) && aligned(state, v) && aligned(w, 16) && aligned(bias, 16) && ldx % 4 == 0 && ldo % 4 == 0 && state_stride % 4 == 0 && D % 4 == 0;
   return FR_B200_OK;
 }
 
-// ---- the selective state space scan ------------------------------------------------------------------------------
-//   delta = softplus(dt + dt_bias)      h[d, n] <- exp(delta[d] A[d, n]) h[d, n] + delta[d] x[d] B[g(d), n]
-//   y[d] = (sum_n C[g(d), n] h[d, n] + D[d] x[d]) * silu(z[d])           g(d) = d / (channels / groups)
-struct SsmArgs {
-  const void *x, *dt, *B, *C, *z;
-  void *out;
-  const float *A, *D, *dt_bias;
-  float *state, *work;
-  long long ldx, lddt, ldb, ldc, ldz, ldo, state_stride;   // elements
-  int d, n, groups, softplus, vec;                         // vec: x, dt, z and out can be taken SSM_VEC channels at a time
-  int shift;                                               // pieces of 2^shift rows
-};
-constexpr int SSM_THREADS = 128, SSM_ROWS = 32;
-
-// A thread has NS states of one channel, L lanes a channel; a CTA walks its 128 / L channels along the rows of a piece, SSM_ROWS at a time:
-// time steps and their products with x are made once per row and channel, and shared.  The sums over a channel's lanes are taken L
-// rows at a time, so that every lane ends with one row's (L - 1 shuffles for L rows).
-//   SSM_WHOLE: the piece is the sequence      SSM_ENDS: the piece's state from zero, and the sum of its time steps
-//   SSM_PIECE: the piece from the state that the pieces before it leave
-enum { SSM_WHOLE = 0, SSM_ENDS = 1, SSM_PIECE = 2 };
-template <typename T, int NS, int L, int MODE>
-__global__ void __launch_bounds__(SSM_THREADS) ssm_seq_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
-  constexpr int CH = SSM_THREADS / L, NP = NS * L, EPT = CH * SSM_ROWS / SSM_THREADS, BPT = NP * SSM_ROWS / SSM_THREADS;
-  constexpr bool BC_AHEAD = BPT <= 8;   // more B and C than this are fetched when they are put down: there is more work to a row then
-  __shared__ float2 s_du[SSM_ROWS][CH];
-  __shared__ __align__(16) float s_b[SSM_ROWS][NP], s_c[SSM_ROWS][NP];
-  __shared__ float s_y[SSM_ROWS][CH + 1];
-  const int tid = threadIdx.x;
-  int s, piece = 0;
-  long long row, end;
-  if (MODE == SSM_WHOLE) {
-    s = blockIdx.y; row = tab.first[s]; end = tab.first[s + 1];
-  } else {
-    s = seq_of(tab, blockIdx.y, a.shift);
-    piece = blockIdx.y - seq_key(tab, s, a.shift);
-    row = tab.first[s] + ((long long)piece << a.shift);
-    end = tab.first[s + 1];
-    if (piece > 0 && row >= end) return;
-    if (end - row > (1ll << a.shift)) end = row + (1ll << a.shift);
-    if (MODE == SSM_ENDS && end == tab.first[s + 1]) return;   // nobody follows the last piece
-  }
-  const bool last = MODE == SSM_WHOLE || end == tab.first[s + 1];
-  // the channels of a CTA are of one group
-  const int per_group = a.d / a.groups, ctas = (per_group + CH - 1) / CH, group = blockIdx.x / ctas;
-  const int ch0 = group * per_group + (blockIdx.x - group * ctas) * CH, ch_end = (group + 1) * per_group;
-  const int ch = ch0 + tid / L, n0 = (tid % L) * NS;
-  const bool live = ch < ch_end;
-
-  float A2[NS], h[NS];
-  const float *slot = nullptr;
-  float *work = nullptr;
-  const size_t dn = (size_t)a.d * a.n;
-  if (MODE != SSM_WHOLE) work = a.work + (size_t)blockIdx.y * (dn + a.d);
-  if (MODE == SSM_WHOLE) { if (tab.from[s] >= 0) slot = a.state + tab.from[s] * a.state_stride; }
-  else if (MODE == SSM_PIECE) slot = work;
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    const bool there = live && n0 + i < a.n;
-    A2[i] = there ? a.A[(size_t)ch * a.n + n0 + i] * LOG2E : 0.f;
-    h[i] = there && slot ? slot[(size_t)ch * a.n + n0 + i] : 0.f;
-  }
-  // what a thread puts down: EPT channels of one row
-  constexpr int TPR = CH / EPT;
-  const int lr = tid / TPR, lc = (tid % TPR) * EPT, gc = ch0 + lc;
-  const int ln = ch_end - gc < EPT ? (ch_end - gc > 0 ? ch_end - gc : 0) : EPT;
-  const bool whole = a.vec && ln == EPT;
-  float bias[EPT], skip[EPT];
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    bias[i] = i < ln && a.dt_bias ? a.dt_bias[gc + i] : 0.f;
-    skip[i] = i < ln && a.D && MODE != SSM_ENDS ? a.D[gc + i] : 0.f;
-  }
-  const T *xp = reinterpret_cast<const T *>(a.x) + gc, *dtp = reinterpret_cast<const T *>(a.dt) + gc, *zp = reinterpret_cast<const T *>(a.z) + gc;
-  T *op = reinterpret_cast<T *>(a.out) + gc;
-  const long long goff = (long long)group * a.n;
-  const T *bp = reinterpret_cast<const T *>(a.B) + goff, *cp = reinterpret_cast<const T *>(a.C) + goff;
-
-  Pack<T, EPT> xn, dn_, zn, xc, zc;
-  T bn[BC_AHEAD ? BPT : 1], cn[BC_AHEAD ? BPT : 1];
-  auto fetch = [&](long long r0) {
-    const long long r = r0 + lr;
-    const int n = r < end ? ln : 0;
-    const bool w = whole && r < end;
-    xn = load_pack<T, EPT>(xp + r * a.ldx, n, w);
-    dn_ = load_pack<T, EPT>(dtp + r * a.lddt, n, w);
-    if (MODE != SSM_ENDS && a.z) zn = load_pack<T, EPT>(zp + r * a.ldz, n, w);
-    if (BC_AHEAD)
-#pragma unroll
-      for (int q = 0; q < BPT; ++q) {
-        const int e = tid + q * SSM_THREADS, er = e / NP, en = e % NP;
-        const bool there = r0 + er < end && en < a.n;
-        bn[q] = there ? bp[(r0 + er) * a.ldb + en] : from_f<T>(0.f);
-        if (MODE != SSM_ENDS) cn[q] = there ? cp[(r0 + er) * a.ldc + en] : from_f<T>(0.f);
-      }
-  };
-  float dsum[EPT];
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) dsum[i] = 0.f;
-  auto put_down = [&](long long r0) {
-    const bool there = r0 + lr < end;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      float v = to_f(dn_.v[i]) + bias[i];
-      if (a.softplus) v = softplus(v);
-      if (!there || i >= ln) v = 0.f;
-      s_du[lr][lc + i] = make_float2(v, there && i < ln ? v * to_f(xn.v[i]) : 0.f);
-      if (MODE == SSM_ENDS) dsum[i] += v;
-    }
-#pragma unroll 8
-    for (int q = 0; q < BPT; ++q) {
-      const int e = tid + q * SSM_THREADS, er = e / NP, en = e % NP;
-      if (BC_AHEAD) {
-        s_b[er][en] = to_f(bn[q]);
-        if (MODE != SSM_ENDS) s_c[er][en] = to_f(cn[q]);
-      } else {
-        const bool there2 = r0 + er < end && en < a.n;
-        s_b[er][en] = there2 ? to_f(bp[(r0 + er) * a.ldb + en]) : 0.f;
-        if (MODE != SSM_ENDS) s_c[er][en] = there2 ? to_f(cp[(r0 + er) * a.ldc + en]) : 0.f;
-      }
-    }
-  };
-  if (row < end) { fetch(row); put_down(row); }
-  for (; row < end; row += SSM_ROWS) {
-    xc = xn; zc = zn;
-    __syncthreads();
-    if (row + SSM_ROWS < end) fetch(row + SSM_ROWS);
-    const int left = end - row < SSM_ROWS ? (int)(end - row) : SSM_ROWS;
-    for (int t0 = 0; t0 < left; t0 += L) {
-      float p[L];
-      auto one = [&](int k) {
-        const float2 du = s_du[t0 + k][tid / L];
-        const Pack<float, NS> b = *reinterpret_cast<const Pack<float, NS> *>(&s_b[t0 + k][n0]);
-        Pack<float, NS> c;
-        if (MODE != SSM_ENDS) c = *reinterpret_cast<const Pack<float, NS> *>(&s_c[t0 + k][n0]);
-        p[k] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          h[i] = fmaf(ex2(du.x * A2[i]), h[i], du.y * b.v[i]);
-          if (MODE != SSM_ENDS) p[k] = fmaf(h[i], c.v[i], p[k]);
-        }
-      };
-      if (t0 + L <= left) {
-#pragma unroll
-        for (int k = 0; k < L; ++k) one(k);
-      } else {
-        // rows behind the end have no say, whatever exp makes of 0 x A
-#pragma unroll
-        for (int k = 0; k < L; ++k) {
-          p[k] = 0.f;
-          if (t0 + k < left) one(k);
-        }
-      }
-      if (MODE != SSM_ENDS) {
-        const int lane = tid % L;
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) {
-          const bool up = lane & o;
-#pragma unroll
-          for (int k = 0; k < o; ++k) {
-            const float send = up ? p[k] : p[k + o], keep = up ? p[k + o] : p[k];
-            p[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-          }
-        }
-        s_y[t0 + lane][tid / L] = p[0];
-      }
-    }
-    __syncthreads();
-    if (MODE != SSM_ENDS && row + lr < end) {
-      Pack<T, EPT> o;
-#pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        float y = fmaf(skip[i], to_f(xc.v[i]), s_y[lr][lc + i]);
-        if (a.z) y *= silu(to_f(zc.v[i]));
-        o.v[i] = from_f<T>(y);
-      }
-      store_pack<T, EPT>(op + (row + lr) * a.ldo, o, ln, whole);
-    }
-    if (row + SSM_ROWS < end) put_down(row + SSM_ROWS);
-  }
-  if (MODE == SSM_ENDS) {
-    // the sum of a channel's time steps, over the rows' threads in a fixed order
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) s_y[lr][lc + i] = dsum[i];
-    __syncthreads();
-    if (tid < CH && ch0 + tid < ch_end) {
-      float v = 0.f;
-      for (int r = 0; r < SSM_ROWS; ++r) v += s_y[r][tid];
-      work[dn + ch0 + tid] = v;
-    }
-  }
-  float *to = nullptr;
-  if (MODE == SSM_ENDS) to = work;
-  else if (last && tab.to[s] >= 0) to = a.state + tab.to[s] * a.state_stride;
-  if (to)
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (live && n0 + i < a.n) to[(size_t)ch * a.n + n0 + i] = h[i];
-}
-
-// The pieces' states from zero -> the states that they begin with, in their place: S <- exp(A sum of time steps) S + end.
-// One thread per channel and state of a sequence.
-__global__ void __launch_bounds__(256) ssm_join_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
-  const int e = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y;
-  const size_t dn = (size_t)a.d * a.n;
-  if (e >= (long long)dn) return;
-  const long long len = tab.first[s + 1] - tab.first[s];
-  const int pieces = len > 0 ? (int)((len + (1ll << a.shift) - 1) >> a.shift) : 1, ch = e / a.n;
-  float *w = a.work + (size_t)seq_key(tab, s, a.shift) * (dn + a.d);
-  const float A2 = a.A[e] * LOG2E;
-  float S = tab.from[s] >= 0 ? a.state[tab.from[s] * a.state_stride + e] : 0.f;
-  for (int p = 0; p < pieces; ++p, w += dn + a.d) {
-    float end = 0.f, sum = 0.f;
-    if (p + 1 < pieces) { end = w[e]; sum = w[dn + ch]; }
-    w[e] = S;
-    if (p + 1 < pieces) S = fmaf(ex2(sum * A2), S, end);
-  }
-}
-
-// One token of each stream.  L lanes a channel of four states at a time.
-template <typename T, int L>
+// ---- the selective state space scan (sequences: ssm.cuh) ----------------------------------------------------------
+// One token of each stream: L lanes a channel, four states a lane (and every 4 L-th four), CPT channels a thread, whose states are all asked
+// for at once.  Bound by reading and writing the states.
+template <typename T, int L, int CPT, bool VEC>
 __global__ void __launch_bounds__(128) ssm_step_kernel(const SsmArgs a, const __grid_constant__ SlotTable tab) {
-  const int lane = threadIdx.x % L, ch = blockIdx.x * (128 / L) + threadIdx.x / L, s = blockIdx.y;
-  const bool live = ch < a.d;
+  constexpr int CH = 128 / L;
+  const int lane = threadIdx.x % L, s = blockIdx.y;
+  // the channels of a CTA are of one group
+  const int per_group = a.d / a.groups, ctas = (per_group + CH * CPT - 1) / (CH * CPT), group = blockIdx.x / ctas;
+  const int ch_end = (group + 1) * per_group, ch0 = group * per_group + (blockIdx.x - group * ctas) * (CH * CPT) + threadIdx.x / L;
   const long long row = tab.base + s;
-  const int c = live ? ch : a.d - 1;
-  const float x = to_f(reinterpret_cast<const T *>(a.x)[row * a.ldx + c]);
-  float delta = to_f(reinterpret_cast<const T *>(a.dt)[row * a.lddt + c]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
-  const long long g = (long long)(c / (a.d / a.groups)) * a.n;
-  const T *bp = reinterpret_cast<const T *>(a.B) + row * a.ldb + g, *cp = reinterpret_cast<const T *>(a.C) + row * a.ldc + g;
-  const float *from = tab.from[s] >= 0 ? a.state + tab.from[s] * a.state_stride + (size_t)c * a.n : nullptr;
-  float *to = tab.to[s] >= 0 ? a.state + tab.to[s] * a.state_stride + (size_t)c * a.n : nullptr;
-  const float *A = a.A + (size_t)c * a.n;
-  if (a.softplus) delta = softplus(delta);
-  const float u = delta * x;
-  float y = 0.f;
-  for (int n = lane * 4; n < a.n; n += 4 * L) {
-    const int k = a.n - n < 4 ? a.n - n : 4;
-    const bool whole = a.vec && k == 4;
-    Pack<float, 4> h, A4 = load_pack<float, 4>(A + n, k, whole);
-    if (from) h = load_pack<float, 4>(from + n, k, whole);
-    else h.v[0] = h.v[1] = h.v[2] = h.v[3] = 0.f;
+  const int from_slot = tab.from[s], to_slot = tab.to[s];
+  pdl_wait();
+  pdl_trigger();
+  const float *from = a.state + (long long)max(from_slot, 0) * a.state_stride;
+  float *to = a.state + (long long)max(to_slot, 0) * a.state_stride;
+  const T *bp = reinterpret_cast<const T *>(a.B) + row * a.ldb + (long long)group * a.n;
+  const T *cp = reinterpret_cast<const T *>(a.C) + row * a.ldc + (long long)group * a.n;
+  const T *zp = a.z ? reinterpret_cast<const T *>(a.z) + row * a.ldz : reinterpret_cast<const T *>(a.x) + row * a.ldx;
+  int c[CPT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < k) {
-        h.v[i] = fmaf(ex2(delta * A4.v[i] * LOG2E), h.v[i], u * to_f(bp[n + i]));
-        y = fmaf(h.v[i], to_f(cp[n + i]), y);
+  for (int k = 0; k < CPT; ++k) c[k] = min(ch0 + k * CH, ch_end - 1);   // (channels past the end: computed, not kept)
+  float y[CPT], x[CPT], delta[CPT], z[CPT], skip[CPT];
+  for (int n = min(lane * 4, a.n - 1), first = 1; n < a.n && lane * 4 < a.n; n += 4 * L, first = 0) {
+    const int left = min(a.n - n, 4);
+    Pack<float, 4> h[CPT], A4[CPT];
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[k].v[i] = 0.f;
+      if (from_slot >= 0) h[k] = load_pack<float, 4, VEC>(from + (size_t)c[k] * a.n + n, left);
+    }
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) A4[k] = load_pack<float, 4, VEC>(a.A + (size_t)c[k] * a.n + n, left);
+    const Pack<T, 4> B = load_pack<T, 4, false>(bp + n, left), C = load_pack<T, 4, false>(cp + n, left);
+    if (first)
+#pragma unroll
+      for (int k = 0; k < CPT; ++k) {
+        x[k] = to_f(reinterpret_cast<const T *>(a.x)[row * a.ldx + c[k]]);
+        float d = to_f(reinterpret_cast<const T *>(a.dt)[row * a.lddt + c[k]]) + (a.dt_bias ? a.dt_bias[c[k]] : 0.f);
+        z[k] = to_f(zp[c[k]]);
+        skip[k] = a.D ? a.D[c[k]] : 0.f;
+        delta[k] = a.softplus ? softplus(d) : d;
+        y[k] = 0.f;
       }
-    if (to && live) store_pack<float, 4>(to + n, h, k, whole);
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+      const float d = delta[k] * LOG2E, u = delta[k] * x[k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        h[k].v[i] = fmaf(ex2(d * A4[k].v[i]), h[k].v[i], u * to_f(B.v[i]));
+        if (i < left) y[k] = fmaf(h[k].v[i], to_f(C.v[i]), y[k]);
+      }
+      if (to_slot >= 0 && ch0 + k * CH < ch_end) store_pack<float, 4, VEC>(to + (size_t)c[k] * a.n + n, h[k], left);
+    }
   }
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (lane == 0 && live) {
-    if (a.D) y = fmaf(a.D[c], x, y);
-    if (a.z) y *= silu(to_f(reinterpret_cast<const T *>(a.z)[row * a.ldz + c]));
-    reinterpret_cast<T *>(a.out)[row * a.ldo + c] = from_f<T>(y);
+  for (int k = 0; k < CPT; ++k) {
+    if (lane * 4 >= a.n) y[k] = x[k] = z[k] = skip[k] = 0.f;   // a lane without states
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+    y[k] = fmaf(skip[k], x[k], y[k]);
+    if (a.z) y[k] *= silu(z[k]);
+    if (lane == 0 && ch0 + k * CH < ch_end) reinterpret_cast<T *>(a.out)[row * a.ldo + c[k]] = from_f<T>(y[k]);
   }
 }
 
-template <typename T, int NS, int L>
-cudaError_t ssm_seq_launch(const SsmArgs &a, const SeqTable &t, bool split, cudaStream_t st) {
-  constexpr int CH = SSM_THREADS / L;
-  const unsigned gx = (a.d / a.groups + CH - 1) / CH * a.groups;
-  if (!split) {
-    ssm_seq_kernel<T, NS, L, SSM_WHOLE><<<dim3(gx, t.n), SSM_THREADS, 0, st>>>(a, t);
-    return cudaGetLastError();
-  }
-  const dim3 grid(gx, seq_items(t, a.shift));
-  ssm_seq_kernel<T, NS, L, SSM_ENDS><<<grid, SSM_THREADS, 0, st>>>(a, t);
-  ssm_join_kernel<<<dim3((unsigned)(((size_t)a.d * a.n + 255) / 256), t.n), 256, 0, st>>>(a, t);
-  ssm_seq_kernel<T, NS, L, SSM_PIECE><<<grid, SSM_THREADS, 0, st>>>(a, t);
-  return cudaGetLastError();
-}
-// the fewest lanes of up to four states that hold N of them
-template <typename T>
-cudaError_t ssm_seq_any(const SsmArgs &a, const SeqTable &t, bool split, cudaStream_t st) {
-  if (a.n <= 8) return ssm_seq_launch<T, 2, 4>(a, t, split, st);
-  if (a.n <= 16) return ssm_seq_launch<T, 4, 4>(a, t, split, st);
-  if (a.n <= 32) return ssm_seq_launch<T, 4, 8>(a, t, split, st);
-  if (a.n <= 64) return ssm_seq_launch<T, 4, 16>(a, t, split, st);
-  return ssm_seq_launch<T, 4, 32>(a, t, split, st);
-}
-template <typename T, int L>
+// four channels a thread where that leaves every SM a few CTAs, else one
+template <typename T, int L, bool VEC>
 cudaError_t ssm_step_launch(const SsmArgs &a, const SlotTable &t, cudaStream_t st) {
-  ssm_step_kernel<T, L><<<dim3((a.d + 128 / L - 1) / (128 / L), t.n), 128, 0, st>>>(a, t);
-  return cudaGetLastError();
+  constexpr int CH = 128 / L;
+  const int per_group = a.d / a.groups;
+  auto grid = [&](int ch) { return dim3((per_group + ch - 1) / ch * a.groups, t.n); };
+  if ((long long)a.d * t.n >= 148ll * 4 * 4 * CH) return op_launch(ssm_step_kernel<T, L, 4, VEC>, grid(4 * CH), 128, 0, st, 1, a, t);
+  return op_launch(ssm_step_kernel<T, L, 1, VEC>, grid(CH), 128, 0, st, 1, a, t);
 }
-template <typename T>
+template <typename T, bool VEC>
 cudaError_t ssm_step_any(const SsmArgs &a, const SlotTable &t, cudaStream_t st) {
-  if (a.n <= 4) return ssm_step_launch<T, 1>(a, t, st);
-  if (a.n <= 8) return ssm_step_launch<T, 2>(a, t, st);
-  if (a.n <= 16) return ssm_step_launch<T, 4>(a, t, st);
-  if (a.n <= 32) return ssm_step_launch<T, 8>(a, t, st);
-  return ssm_step_launch<T, 16>(a, t, st);
+  if (a.n <= 4) return ssm_step_launch<T, 1, VEC>(a, t, st);
+  if (a.n <= 8) return ssm_step_launch<T, 2, VEC>(a, t, st);
+  if (a.n <= 16) return ssm_step_launch<T, 4, VEC>(a, t, st);
+  if (a.n <= 32) return ssm_step_launch<T, 8, VEC>(a, t, st);
+  return ssm_step_launch<T, 16, VEC>(a, t, st);
 }
 
 constexpr int SSM_STATES = 128;   // most states of a channel
@@ -573,14 +356,19 @@ int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots) {
 
 // Pieces of 2^shift rows, or 0: sequences whole.
 int ssm_split(int64_t rows, int n_seq, int d, int n) {
-  (void)rows; (void)n_seq; (void)d; (void)n;
-  return 0;
+  (void)n;
+  // few channels and sequences: one of 4096 rows and 256 channels 231 us whole, 57 in pieces of 256 rows
+  const int64_t ctas = (int64_t)((d + 31) / 32) * n_seq;
+  return ctas <= 40 && rows / n_seq >= 1024 ? 8 : 0;
 }
 
 // ---- slots ------------------------------------------------------------------------------------------------------
-// pool[dst[i]] <- pool[src[i]], as if every source were read before any slot is written; src -1: zeros.  A CTA has `cols` units of every
-// slot of the call to itself: it brings those of the sources into shared memory, then writes them to the slots that take them.
-constexpr int COPY_CAP = 4096, COPY_SMALL = 64, COPY_THREADS = 256;
+// pool[dst[i]] <- pool[src[i]], as if every source were read before any slot is written; src -1: zeros.  A CTA has a column of 16 x cols bytes of every
+// slot of the call to itself: it brings those of the sources into shared memory, then writes them to the slots that take them.  Both
+// sides go by the 16-byte words of memory; where slots begin between them (GRAN < 16: the granule they all are multiples of), a
+// source's words lie in shared memory as they lay, and a word to be written is cut out of two of them.
+// Bound by the bytes: every source once, every destination once.
+constexpr int COPY_CAP = 4096, COPY_SMALL = 64, COPY_THREADS = 256, COPY_SMEM = 96 * 1024;
 template <int CAP>
 struct CopyTable {
   int n_src, n_dst;
@@ -589,65 +377,107 @@ struct CopyTable {
 struct CopyArgs {
   uint8_t *pool;
   size_t stride;     // bytes between slots
-  long long units;   // of a slot
-  int cols;          // units of a CTA
+  long long bytes;   // of a slot
+  int log_cols;      // words of a CTA's column, whole ones
 };
-template <typename U, int CAP>
+template <int GRAN, int CAP>
 __global__ void __launch_bounds__(COPY_THREADS) slots_copy_kernel(const CopyArgs a, const __grid_constant__ CopyTable<CAP> t) {
   extern __shared__ __align__(16) uint8_t copy_smem[];
-  U *s = reinterpret_cast<U *>(copy_smem);
-  const long long c0 = (long long)blockIdx.x * a.cols;
-  const int cols = a.units - c0 < a.cols ? (int)(a.units - c0) : a.cols;
-  const int n_in = t.n_src * a.cols, n_out = t.n_dst * a.cols;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < n_in; e += COPY_THREADS) {
-    const int r = e / a.cols, c = e - r * a.cols;
-    if (c < cols) s[e] = reinterpret_cast<const U *>(a.pool + t.src[r] * a.stride)[c0 + c];
+  const int cols = 1 << a.log_cols, col = threadIdx.x & (cols - 1), row0 = threadIdx.x >> a.log_cols, rows = COPY_THREADS >> a.log_cols;
+  constexpr int MORE = GRAN < 16;                  // a column of unaligned bytes touches one word more
+  const int pitch = (cols + 2 * MORE) * 16;
+  const long long c0 = (long long)blockIdx.x * cols * 16;
+  const int len = (int)min(a.bytes - c0, (long long)cols * 16);
+  pdl_wait();
+  pdl_trigger();
+  constexpr int AT_ONCE = 8;
+  for (int r0 = row0; r0 < t.n_src; r0 += rows * AT_ONCE) {
+    uint4 v[AT_ONCE], more[AT_ONCE];
+#pragma unroll
+    for (int q = 0; q < AT_ONCE; ++q) {
+      const uintptr_t p = reinterpret_cast<uintptr_t>(a.pool) + t.src[min(r0 + q * rows, t.n_src - 1)] * a.stride + c0;
+      const uint4 *w = reinterpret_cast<const uint4 *>(p & ~(uintptr_t)15);
+      const int last = (int)(((p & 15) + len - 1) >> 4);   // the last word with a byte of the column
+      v[q] = w[min(col, last)];
+      if (MORE && col == 0) more[q] = w[min(cols, last)];
+    }
+#pragma unroll
+    for (int q = 0; q < AT_ONCE; ++q)
+      if (r0 + q * rows < t.n_src) {
+        uint4 *s = reinterpret_cast<uint4 *>(copy_smem + (size_t)(r0 + q * rows) * pitch);
+        s[col] = v[q];
+        if (MORE && col == 0) s[cols] = more[q];
+      }
   }
   __syncthreads();
 #pragma unroll 4
-  for (int e = threadIdx.x; e < n_out; e += COPY_THREADS) {
-    const int r = e / a.cols, c = e - r * a.cols;
-    if (c < cols) reinterpret_cast<U *>(a.pool + t.dst[r] * a.stride)[c0 + c] = t.from[r] < t.n_src ? s[t.from[r] * a.cols + c] : U{};
+  for (int r = row0; r < t.n_dst; r += rows) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a.pool) + t.dst[r] * a.stride + c0;
+    const bool zero = t.from[r] >= t.n_src;
+    const uint8_t *s = copy_smem + (size_t)(zero ? 0 : t.from[r]) * pitch;
+    if (GRAN >= 16) {
+      if (col * 16 < len) reinterpret_cast<uint4 *>(p)[col] = zero ? uint4{} : reinterpret_cast<const uint4 *>(s)[col];
+    } else {
+      const int off = (int)(p & 15);
+      const int in = zero ? 0 : (int)((reinterpret_cast<uintptr_t>(a.pool) + t.src[t.from[r]] * a.stride + c0) & 15);
+      for (int w = col; w * 16 < off + len; w += cols) {
+        const int at = w * 16 - off;               // the word's bytes at .. at + 15 of the column
+        uint32_t o[4];
+        const int from = at + in, shift = (from & 3) * 8;
+        const uint32_t *sw = reinterpret_cast<const uint32_t *>(s) + (from >> 2);   // (from >= -15: words before the row's are not taken)
+        uint32_t lo = from >= 0 ? sw[0] : 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t hi = from + 4 * q + 4 >= 0 && (GRAN < 4 || q < 3) ? sw[q + 1] : 0;
+          o[q] = zero ? 0 : GRAN >= 4 ? lo : __funnelshift_r(lo, hi, shift);
+          lo = hi;
+        }
+        uint8_t *d = reinterpret_cast<uint8_t *>(p) + at;
+        if (at >= 0 && at + 16 <= len) *reinterpret_cast<uint4 *>(d) = make_uint4(o[0], o[1], o[2], o[3]);
+        else
+#pragma unroll
+          for (int g = 0; g < 16; g += GRAN)
+            if (at + g >= 0 && at + g < len) {
+              const uint32_t word = o[g / 4] >> (g % 4 * 8);
+              if (GRAN >= 4) *reinterpret_cast<uint32_t *>(d + g) = word;
+              else if (GRAN == 2) *reinterpret_cast<uint16_t *>(d + g) = (uint16_t)word;
+              else d[g] = (uint8_t)word;
+            }
+      }
+    }
   }
 }
-struct U16 { uint32_t x, y, z, w; };
 
-template <typename U, int CAP>
-cudaError_t slots_copy_launch(CopyArgs a, size_t bytes, const CopyTable<CAP> &t, cudaStream_t st) {
-  a.units = (long long)(bytes / sizeof(U));
-  constexpr int SMEM = 64 * 1024;
-  const int rows = t.n_src > 0 ? t.n_src : 1;
-  int cols = SMEM / (int)(rows * sizeof(U));
-  if (cols > COPY_THREADS) cols = COPY_THREADS;
-  if (cols < 1) cols = 1;
-  a.cols = cols;
-  const int smem = (int)(t.n_src * cols * sizeof(U));
-  static thread_local uint64_t told = 0;   // devices whose attribute is set
-  int dev;
-  cudaError_t e = cudaGetDevice(&dev);
+template <int GRAN, int CAP>
+cudaError_t slots_copy_launch(CopyArgs a, const CopyTable<CAP> &t, cudaStream_t st) {
+  const int more = GRAN < 16 ? 2 : 0, rows = t.n_src > 0 ? t.n_src : 1;
+  const long long words = (a.bytes + 15) / 16;
+  // as wide as shared memory takes the sources (some dozen of them: 2 CTAs an SM), but four CTAs for every SM, down to 64 bytes
+  a.log_cols = 8;
+  while (a.log_cols > 0 && (long long)rows * ((1 << a.log_cols) + more) * 16 > COPY_SMEM) --a.log_cols;
+  while (a.log_cols > 2 && (words >> a.log_cols) < 4 * device_sm_count()) --a.log_cols;
+  const int cols = 1 << a.log_cols;
+  const size_t smem = (size_t)t.n_src * (cols + more) * 16 + 16;
+  static thread_local uint64_t told = 0;
+  cudaError_t e = allow_smem(slots_copy_kernel<GRAN, CAP>, 227 * 1024, told);
   if (e != cudaSuccess) return e;
-  if (dev > 63 || !(told >> dev & 1)) {
-    if ((e = cudaFuncSetAttribute(slots_copy_kernel<U, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) != cudaSuccess) return e;
-    if (dev <= 63) told |= 1ull << dev;
-  }
-  slots_copy_kernel<U, CAP><<<(unsigned)((a.units + cols - 1) / cols), COPY_THREADS, smem, st>>>(a, t);
-  return cudaGetLastError();
+  return op_launch(slots_copy_kernel<GRAN, CAP>, dim3((unsigned)((words + cols - 1) >> a.log_cols)), COPY_THREADS, smem, st, 1, a, t);
 }
-// units as wide as the pool's address, its slots and their distance allow
 template <int CAP>
-cudaError_t slots_copy_any(const CopyArgs &a, size_t bytes, const CopyTable<CAP> &t, cudaStream_t st) {
-  const size_t m = reinterpret_cast<uintptr_t>(a.pool) | a.stride | bytes;
-  if (m % 16 == 0) return slots_copy_launch<U16>(a, bytes, t, st);
-  if (m % 4 == 0) return slots_copy_launch<uint32_t>(a, bytes, t, st);
-  if (m % 2 == 0) return slots_copy_launch<uint16_t>(a, bytes, t, st);
-  return slots_copy_launch<uint8_t>(a, bytes, t, st);
+cudaError_t slots_copy_any(const CopyArgs &a, const CopyTable<CAP> &t, cudaStream_t st) {
+  const size_t m = reinterpret_cast<uintptr_t>(a.pool) | a.stride | (size_t)a.bytes;
+  if (m % 16 == 0) return slots_copy_launch<16>(a, t, st);
+  if (m % 4 == 0) return slots_copy_launch<4>(a, t, st);
+  if (m % 2 == 0) return slots_copy_launch<2>(a, t, st);
+  return slots_copy_launch<1>(a, t, st);
 }
 // dst[e] = value for e < n of `layers` vectors, layer_stride bytes apart, in each of the slots that the table clears
 template <int CAP>
 __global__ void __launch_bounds__(COPY_THREADS) slots_fill_kernel(uint8_t *at, size_t stride, size_t layer_stride, int n, float value,
                                                                   const __grid_constant__ CopyTable<CAP> t) {
   const int e = blockIdx.x * COPY_THREADS + threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
   if (e < n && t.from[blockIdx.z] == t.n_src) reinterpret_cast<float *>(at + t.dst[blockIdx.z] * stride + blockIdx.y * layer_stride)[e] = value;
 }
 
@@ -667,14 +497,13 @@ cudaError_t slots_copy_moves(uint8_t *pool, size_t bytes, size_t stride, int n_s
     t.from[t.n_dst++] = (uint16_t)(src[i] < 0 ? t.n_src : place[src[i]]);
   }
   if (!t.n_dst) return cudaSuccess;
-  cudaError_t e = slots_copy_any(CopyArgs{pool, stride, 0, 0}, bytes, t, st);
+  cudaError_t e = slots_copy_any(CopyArgs{pool, stride, (long long)bytes, 0}, t, st);
   if (e != cudaSuccess || !fill) return e;
   bool clears = false;
   for (int i = 0; i < t.n_dst; ++i) clears |= t.from[i] == t.n_src;
   if (!clears) return e;
-  slots_fill_kernel<CAP><<<dim3((fill->n + COPY_THREADS - 1) / COPY_THREADS, fill->layers, t.n_dst), COPY_THREADS, 0, st>>>(
-      pool + fill->offset, stride, fill->layer_stride, fill->n, fill->value, t);
-  return cudaGetLastError();
+  return op_launch(slots_fill_kernel<CAP>, dim3((fill->n + COPY_THREADS - 1) / COPY_THREADS, fill->layers, t.n_dst), COPY_THREADS, 0, st, 1,
+                   pool + fill->offset, stride, fill->layer_stride, fill->n, fill->value, t);
 }
 
 }  // namespace
@@ -748,15 +577,16 @@ int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, co
                     const int32_t *from, const int32_t *to, void *out, int64_t ldo, void *work, size_t work_bytes, int device, void *stream) {
   OP_TRY
   SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, reinterpret_cast<float *>(work), ldx, lddt, ldb, ldc, ldz, ldo, state_stride,
-            D, N, groups, dt_softplus != 0, 0, 0};
+            D, N, groups, dt_softplus != 0, 0, 0, 0};
   int rc;
   if ((rc = ssm_check(a, dtype, rows, n_slots))) return rc;
   if ((rc = check_starts(starts, n_seq, rows)) || (rc = check_slots(n_seq, state, n_slots, from, to))) return rc;
   if (n_seq == 0) return FR_B200_OK;
-  const size_t v = 8 * (size_t)dt_bytes(dtype) < 16 ? 8 * (size_t)dt_bytes(dtype) : 16;
+  const size_t v = 8 * (size_t)dt_bytes(dtype);   // a thread's piece of a row: up to eight channels
   a.vec = aligned(x, v) && aligned(dt, v) && aligned(z, v) && aligned(out, v) && ldx % 8 == 0 && lddt % 8 == 0 && (!z || ldz % 8 == 0) && ldo % 8 == 0 &&
           (D / groups) % 8 == 0;
   a.shift = rows > 0 ? ssm_split(rows, n_seq, D, N) : 0;
+  a.wide = (int64_t)((D / groups + 63) / 64) * groups * n_seq >= 400;   // 64 channels a CTA: some for every SM (640 CTAs 176 us against 189, 128 200 against 165)
   const size_t need = fr_b200_ssm_seq_workspace(rows, n_seq, D, N);
   OP_REQUIRE(work_bytes >= need && (!need || (work && aligned(work, 4))), "the work area is smaller than fr_b200_ssm_seq_workspace()");
   DeviceScope dev;
@@ -765,9 +595,9 @@ int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, co
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   for (int i = 0; i < n_seq; i += SEQ_CAP) {
     fill_table(t, i, n_seq, starts, rows, state, from, to);
-    if (dtype == FR_B200_T_F16) OP_CU(ssm_seq_any<__half>(a, t, need > 0, st));
-    else if (dtype == FR_B200_T_BF16) OP_CU(ssm_seq_any<__nv_bfloat16>(a, t, need > 0, st));
-    else OP_CU(ssm_seq_any<float>(a, t, need > 0, st));
+    if (dtype == FR_B200_T_F16) OP_CU(launch_ssm_seq<__half>(a, t, st));
+    else if (dtype == FR_B200_T_BF16) OP_CU(launch_ssm_seq<__nv_bfloat16>(a, t, st));
+    else OP_CU(launch_ssm_seq<float>(a, t, st));
   }
   return FR_B200_OK;
   OP_CATCH
@@ -778,7 +608,7 @@ int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, c
                      int N, int groups, float *state, int64_t state_stride, int n_slots, const int32_t *from, const int32_t *to, void *out,
                      int64_t ldo, int device, void *stream) {
   OP_TRY
-  SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, nullptr, ldx, lddt, ldb, ldc, ldz, ldo, state_stride, D, N, groups, dt_softplus != 0, 0, 0};
+  SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, nullptr, ldx, lddt, ldb, ldc, ldz, ldo, state_stride, D, N, groups, dt_softplus != 0, 0, 0, 0};
   int rc;
   if ((rc = ssm_check(a, dtype, n, n_slots)) || (rc = check_slots(n, state, n_slots, from, to))) return rc;
   a.vec = aligned(state, 16) && aligned(A, 16) && state_stride % 4 == 0 && N % 4 == 0;
@@ -788,9 +618,9 @@ int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, c
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   for (int i = 0; i < n; i += SLOT_CAP) {
     fill_slots(t, i, n, state, from, to);
-    if (dtype == FR_B200_T_F16) OP_CU(ssm_step_any<__half>(a, t, st));
-    else if (dtype == FR_B200_T_BF16) OP_CU(ssm_step_any<__nv_bfloat16>(a, t, st));
-    else OP_CU(ssm_step_any<float>(a, t, st));
+    if (dtype == FR_B200_T_F16) OP_CU((a.vec ? ssm_step_any<__half, true> : ssm_step_any<__half, false>)(a, t, st));
+    else if (dtype == FR_B200_T_BF16) OP_CU((a.vec ? ssm_step_any<__nv_bfloat16, true> : ssm_step_any<__nv_bfloat16, false>)(a, t, st));
+    else OP_CU((a.vec ? ssm_step_any<float, true> : ssm_step_any<float, false>)(a, t, st));
   }
   return FR_B200_OK;
   OP_CATCH

@@ -1,0 +1,4 @@
+#define FRB_SSM_KERNELS
+#include "ssm.cuh"
+
+template cudaError_t frb::launch_ssm_seq<__half>(const SsmArgs &, const SeqTable &, cudaStream_t);
