@@ -496,6 +496,48 @@ def test_model_copy_states(pkg, synth, shape_name, strategy):
     m.close()
 
 
+# ---- what does not fit together ----------------------------------------------------------------------------------
+
+def test_tensors_that_do_not_fit_are_refused(pkg):
+    x, w, b = _rand(4, 64, dtype=F16), _rand(32, 64, dtype=F16), _rand(32)
+    cw, pool = _rand(64, 4), _rand(6, 3, 64, dtype=F16)
+    A, B, ssm = _rand(64, 8), _rand(4, 16, dtype=F16), _rand(6, 64, 8)
+    no = [lambda: pkg.linear(x, w.bfloat16()), lambda: pkg.linear(x, w.cpu()), lambda: pkg.linear(x, w[:, :60]), lambda: pkg.linear(x.t(), w), lambda: pkg.linear(x[0], w),
+          lambda: pkg.linear(x, w, b.half()), lambda: pkg.linear(x, w, b[:31]), lambda: pkg.linear(x, w, residual=_rand(4, 32)), lambda: pkg.linear(x, w, residual=_rand(5, 32, dtype=F16)),
+          lambda: pkg.linear(x, w, out=_rand(4, 31, dtype=F16)), lambda: pkg.linear(x, w, out_dtype=torch.float64), lambda: pkg.linear(x, w, out_dtype="f32"),
+          lambda: pkg.linear(x.double(), w.double()), lambda: pkg.conv_step(x, cw[:, 0]), lambda: pkg.conv_step(x, cw.t()), lambda: pkg.conv_step(x, cw, state=pool.float()),
+          lambda: pkg.conv_step(x, cw, state=pool[:, :2]), lambda: pkg.conv_step(x, cw, state=pool.transpose(1, 2)), lambda: pkg.conv_step(x, cw, state=pool, from_slots=[0, 1, 2]),
+          lambda: pkg.conv_step(x, cw, state=pool, from_slots=[0, 1, 2, 1.5]), lambda: pkg.conv_step(x, cw, state=pool, to_slots=[0, 1, 2, 1 << 40]),
+          lambda: pkg.conv_step(x, cw, state=pool, to_slots=torch.arange(4, device="cuda")), lambda: pkg.conv_step(x, cw, state=pool, to_slots=np.zeros((4, 1), np.int32)),
+          lambda: pkg.conv_seq(x, cw, starts=[]), lambda: pkg.conv_seq(x, cw, starts="12"), lambda: pkg.ssm_step(x, x, A, B, B[:, :8]), lambda: pkg.ssm_step(x, x, A, B[:, :12], B[:, :12]),
+          lambda: pkg.ssm_step(x, x[:, :32], A, B, B), lambda: pkg.ssm_step(x, x.float(), A, B, B), lambda: pkg.ssm_step(x, x, A[:60], B, B), lambda: pkg.ssm_step(x, x, A, B[:3], B[:3]),
+          lambda: pkg.ssm_step(x, x, A, B, B, z=x[:3]), lambda: pkg.ssm_step(x, x, A, B, B, state=ssm.half()), lambda: pkg.ssm_seq(x, x, A, B, B, D=_rand(63)),
+          lambda: pkg.copy_slots(pool.transpose(1, 2), [0], [1]), lambda: pkg.copy_slots(pool, [0, 1], [1]), lambda: pkg.copy_slots(pool, None, [1]), lambda: pkg.copy_slots(pool, [0], 1)]
+    for i, f in enumerate(no):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was taken")
+    lib = [lambda: pkg.linear(x.float(), w.float()), lambda: pkg.linear(x, w, out=x[:, :32]), lambda: pkg.conv_step(x, cw, activation="gelu"), lambda: pkg.conv_step(x, cw, out=x),
+           lambda: pkg.conv_step(x, cw, state=pool, from_slots=[0, 1, 2, 6]), lambda: pkg.conv_step(x, cw, state=pool, to_slots=[0, 1, 2, 2]), lambda: pkg.conv_seq(x, cw, starts=[0, 5]),
+           lambda: pkg.conv_seq(x, cw, starts=[3, 1]), lambda: pkg.conv_seq(x, cw, from_slots=[0]), lambda: pkg.ssm_seq(x, x.clone(), A, B, B, out=x),
+           lambda: pkg.ssm_step(x, x, A, B, B, state=ssm[:3]), lambda: pkg.copy_slots(pool, [0, 1], [2, 2]), lambda: pkg.copy_slots(pool, [0], [6])]
+    for i, f in enumerate(lib):
+        with pytest.raises(pkg.FrB200Error):
+            f()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_lists_of_every_kind(pkg):
+    x, w, pool = _rand(3, 8, dtype=F16), _rand(8, 4), _rand(5, 3, 8, dtype=F16)
+    want = pkg.conv_step(x, w, state=pool.clone(), from_slots=[4, -1, 0], to_slots=[3, 1, 2])
+    for f, t in (((4, -1, 0), (3, 1, 2)), (np.array([4, -1, 0], np.int32), np.array([3, 1, 2], np.int64)), (torch.tensor([4, -1, 0]), torch.tensor([3, 1, 2], dtype=torch.int32)),
+                 (np.array([4, 9, -1, 9, 0, 9], np.int32)[::2], [np.int16(3), np.int64(1), 2])):
+        p = pool.clone()
+        assert torch.equal(pkg.conv_step(x, w, state=p, from_slots=f, to_slots=t), want)
+        assert torch.equal(p[3, -1], x[0]) and torch.equal(p[1, -1], x[1]) and torch.equal(p[2, -1], x[2])
+    assert torch.equal(pkg.conv_step(x, w, state=pool, from_slots=-1, to_slots=-1), pkg.conv_step(x, w))
+
+
 # ---- together ----------------------------------------------------------------------------------------------------
 
 class _Layer:

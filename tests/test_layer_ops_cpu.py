@@ -141,16 +141,11 @@ def test_tensors_that_are_refused(pkg):
         pkg.ssm_seq(x, x, x, x, x)
     with pytest.raises(ValueError, match="GPU"):
         pkg.copy_slots(x, [0], [1])
-    ops = pkg.ops
-    for bad in ([[0, 1]], [0.5, 1.0], np.zeros((2, 1), np.int32)):
-        with pytest.raises(ValueError):
-            ops._ints(bad, 2, "slots")
-    with pytest.raises(ValueError, match="entries"):
-        ops._ints([1, 2, 3], 2, "slots")
-    with pytest.raises(ValueError, match="32-bit"):
-        ops._ints([1, 1 << 40], 2, "slots")
-    assert ops._ints(-1, 3, "slots")[1].tolist() == [-1, -1, -1]
-    assert ops._ints(np.arange(6)[::2], 3, "slots")[1].tolist() == [0, 2, 4]
+    for bad in ("tanh", None, 3):
+        with pytest.raises(ValueError, match="activation"):
+            pkg.linear(x, x, activation=bad)
+    with pytest.raises(ValueError, match="not a tensor"):
+        pkg.linear([1], x)
 
 
 @pytest.mark.parametrize("seed", range(4))
