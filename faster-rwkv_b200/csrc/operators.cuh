@@ -72,19 +72,23 @@ struct alignas(sizeof(T) * V) Pack { T v[V]; };
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ Pack<T, V> load_pack(const T *p, int n) {
   Pack<T, V> r;
-  if constexpr (VEC) r = *reinterpret_cast<const Pack<T, V> *>(p);
-  else
+  if constexpr (VEC) {
+    r = *reinterpret_cast<const Pack<T, V> *>(p);
+  } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = p[i < n ? i : n - 1];
+  }
   return r;
 }
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n) {
-  if constexpr (VEC) *reinterpret_cast<Pack<T, V> *>(p) = r;
-  else
+  if constexpr (VEC) {
+    *reinterpret_cast<Pack<T, V> *>(p) = r;
+  } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) p[i] = r.v[i];
+  }
 }
 
 __device__ __forceinline__ float ex2(float v) {
@@ -182,18 +186,15 @@ cudaError_t launch_slots_copy(void *pool, size_t bytes, size_t stride, int n_slo
 constexpr int SEQ_CAP = 256;
 struct SeqTable {
   int n;
-  int from[SEQ_CAP], to[SEQ_CAP];   // slots, or -1
-  long long first[SEQ_CAP + 1];     // rows first[i] .. first[i + 1] - 1 are sequence i
+  int from[SEQ_CAP], to[SEQ_CAP];            // slots, or -1
+  long long first[SEQ_CAP], end[SEQ_CAP];    // rows first[i] .. end[i] - 1 are sequence i
+  int key[SEQ_CAP + 1];                      // the number of its first piece of 2^shift rows (at least one: an empty sequence hands its state on)
 };
-// Pieces of 2^shift rows: sequence i has the numbers from seq_key(i) on, at least one and as many as it has pieces; numbers behind
-// them, up to the next sequence's first, are of nobody.  (floor((a + b) / len) + 1 >= floor(a / len) + max(1, ceil(b / len)).)
-__host__ __device__ inline int seq_key(const SeqTable &t, int i, int shift) { return (int)((t.first[i] - t.first[0]) >> shift) + i; }
-inline int seq_items(const SeqTable &t, int shift) { return (int)((t.first[t.n] - t.first[0]) >> shift) + t.n; }
-__device__ inline int seq_of(const SeqTable &t, int item, int shift) {
+__device__ inline int seq_of(const SeqTable &t, int item) {
   int lo = 0, hi = t.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (seq_key(t, mid, shift) <= item) lo = mid;
+    if (t.key[mid] <= item) lo = mid;
     else hi = mid - 1;
   }
   return lo;

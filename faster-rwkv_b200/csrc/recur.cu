@@ -40,14 +40,25 @@ int frb::check_slots(int n, const void *state, int n_slots, const int32_t *from,
 
 namespace {
 
-// rows of the sequences and their slots -> one launch's table, from sequence i0 on
-void fill_table(SeqTable &t, int i0, int n_seq, const int32_t *starts, int64_t rows, const void *state, const int32_t *from, const int32_t *to) {
+// rows of the sequences and their slots -> one launch's table, from sequence i0 on, the longest first (sequences run side by side: what
+// takes longest must not begin last); pieces of 2^shift rows
+void fill_table(SeqTable &t, int i0, int n_seq, const int32_t *starts, int64_t rows, const void *state, const int32_t *from, const int32_t *to, int shift) {
   t.n = n_seq - i0 < SEQ_CAP ? n_seq - i0 : SEQ_CAP;
+  auto first = [&](int i) { return starts ? (long long)starts[i] : 0ll; };
+  auto end = [&](int i) { return starts ? (long long)starts[i + 1] : (long long)rows; };
+  int order[SEQ_CAP];
+  for (int i = 0; i < t.n; ++i) order[i] = i0 + i;
+  std::stable_sort(order, order + t.n, [&](int a, int b) { return end(a) - first(a) > end(b) - first(b); });
+  t.key[0] = 0;
   for (int i = 0; i < t.n; ++i) {
-    t.from[i] = !state ? -1 : from ? from[i0 + i] : i0 + i;
-    t.to[i] = !state ? -1 : to ? to[i0 + i] : i0 + i;
+    const int s = order[i];
+    t.from[i] = !state ? -1 : from ? from[s] : s;
+    t.to[i] = !state ? -1 : to ? to[s] : s;
+    t.first[i] = first(s);
+    t.end[i] = end(s);
+    const long long len = t.end[i] - t.first[i];
+    t.key[i + 1] = t.key[i] + (len > 0 ? (int)((len + (1ll << shift) - 1) >> shift) : 1);
   }
-  for (int i = 0; i <= t.n; ++i) t.first[i] = starts ? starts[i0 + i] : i ? rows : 0;
 }
 int check_starts(const int32_t *starts, int n_seq, int64_t rows) {
   OP_REQUIRE(n_seq >= 0, "a negative number of sequences");
@@ -98,8 +109,8 @@ template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(128) conv_seq_kernel(const ConvArgs a, const __grid_constant__ SeqTable tab) {
   constexpr int V = 4;
   const int c = (blockIdx.y * 128 + threadIdx.x) * V;
-  const int item = blockIdx.x, s = seq_of(tab, item, CONV_SHIFT), piece = item - seq_key(tab, s, CONV_SHIFT);
-  const long long first = tab.first[s], end = tab.first[s + 1], row0 = first + (long long)piece * CONV_ROWS;
+  const int item = blockIdx.x, s = seq_of(tab, item), piece = item - tab.key[s];
+  const long long first = tab.first[s], end = tab.end[s], row0 = first + (long long)piece * CONV_ROWS;
   pdl_wait();
   pdl_trigger();
   if (c >= a.D || (piece > 0 && row0 >= end)) return;
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const ConvArgs a, const 
 
 template <typename T, int W, bool VEC>
 cudaError_t conv_go(const ConvArgs &a, const SeqTable &t, cudaStream_t st) {
-  return op_launch(conv_seq_kernel<T, W, VEC>, dim3(seq_items(t, CONV_SHIFT), (a.D + 511) / 512), 128, 0, st, 1, a, t);
+  return op_launch(conv_seq_kernel<T, W, VEC>, dim3(t.key[t.n], (a.D + 511) / 512), 128, 0, st, 1, a, t);
 }
 template <typename T, int W, bool VEC>
 cudaError_t conv_go(const ConvArgs &a, const SlotTable &t, cudaStream_t st) {
@@ -354,12 +365,14 @@ int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots) {
   return FR_B200_OK;
 }
 
-// Pieces of 2^shift rows, or 0: sequences whole.
-int ssm_split(int64_t rows, int n_seq, int d, int n) {
-  (void)n;
-  // few channels and sequences: one of 4096 rows and 256 channels 231 us whole, 57 in pieces of 256 rows
-  const int64_t ctas = (int64_t)((d + 31) / 32) * n_seq;
-  return ctas <= 40 && rows / n_seq >= 1024 ? 8 : 0;
+// Pieces of 2^shift rows, or 0: sequences whole.  Long sequences of few channels: their pieces side by side, twice the work, as long as that leaves a CTA
+// or two for every SM.  One of 4096 rows and 256 channels 92 us whole, 30 in pieces of 256 rows; of 1536 channels 136 and 130.
+int ssm_split(int64_t rows, int n_seq, int d) {
+  const int64_t units = (int64_t)((d + 31) / 32) * n_seq;
+  if (units > 24 || rows < 1024ll * n_seq) return 0;
+  int shift = 8;
+  while ((rows >> shift) * units > 296) ++shift;
+  return shift;
 }
 
 // ---- slots ------------------------------------------------------------------------------------------------------
@@ -541,7 +554,7 @@ int fr_b200_conv_seq(const void *x, int64_t ldx, int dtype, int64_t rows, int D,
   OP_CU(dev.enter(device));
   SeqTable t;
   for (int i = 0; i < n_seq; i += SEQ_CAP) {
-    fill_table(t, i, n_seq, starts, rows, state, from, to);
+    fill_table(t, i, n_seq, starts, rows, state, from, to, CONV_SHIFT);
     OP_CU(conv_any(dtype, taps, a, t, vec, reinterpret_cast<cudaStream_t>(stream)));
   }
   return FR_B200_OK;
@@ -567,8 +580,8 @@ int fr_b200_conv_step(const void *x, int64_t ldx, int dtype, int n, int D, const
 }
 
 size_t fr_b200_ssm_seq_workspace(int64_t rows, int n_seq, int D, int N) {
-  const int shift = rows > 0 && n_seq > 0 && D > 0 && N > 0 ? ssm_split(rows, n_seq, D, N) : 0;
-  return shift ? ((size_t)(rows >> shift) + (n_seq < SEQ_CAP ? n_seq : SEQ_CAP)) * ((size_t)D * N + D) * 4 : 0;
+  const int shift = rows > 0 && n_seq > 0 && D > 0 && N > 0 ? ssm_split(rows, n_seq, D) : 0;
+  return shift ? ((size_t)(rows >> shift) + n_seq) * ((size_t)D * N + D) * 4 : 0;
 }
 
 int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, const float *A, const void *B, int64_t ldb, const void *C,
@@ -577,7 +590,7 @@ int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, co
                     const int32_t *from, const int32_t *to, void *out, int64_t ldo, void *work, size_t work_bytes, int device, void *stream) {
   OP_TRY
   SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, reinterpret_cast<float *>(work), ldx, lddt, ldb, ldc, ldz, ldo, state_stride,
-            D, N, groups, dt_softplus != 0, 0, 0, 0};
+            D, N, groups, dt_softplus != 0, 0, 0};
   int rc;
   if ((rc = ssm_check(a, dtype, rows, n_slots))) return rc;
   if ((rc = check_starts(starts, n_seq, rows)) || (rc = check_slots(n_seq, state, n_slots, from, to))) return rc;
@@ -585,8 +598,7 @@ int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, co
   const size_t v = 8 * (size_t)dt_bytes(dtype);   // a thread's piece of a row: up to eight channels
   a.vec = aligned(x, v) && aligned(dt, v) && aligned(z, v) && aligned(out, v) && ldx % 8 == 0 && lddt % 8 == 0 && (!z || ldz % 8 == 0) && ldo % 8 == 0 &&
           (D / groups) % 8 == 0;
-  a.shift = rows > 0 ? ssm_split(rows, n_seq, D, N) : 0;
-  a.wide = (int64_t)((D / groups + 63) / 64) * groups * n_seq >= 400;   // 64 channels a CTA: some for every SM (640 CTAs 176 us against 189, 128 200 against 165)
+  a.shift = rows > 0 ? ssm_split(rows, n_seq, D) : 0;
   const size_t need = fr_b200_ssm_seq_workspace(rows, n_seq, D, N);
   OP_REQUIRE(work_bytes >= need && (!need || (work && aligned(work, 4))), "the work area is smaller than fr_b200_ssm_seq_workspace()");
   DeviceScope dev;
@@ -594,7 +606,7 @@ int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, co
   SeqTable t;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   for (int i = 0; i < n_seq; i += SEQ_CAP) {
-    fill_table(t, i, n_seq, starts, rows, state, from, to);
+    fill_table(t, i, n_seq, starts, rows, state, from, to, a.shift);
     if (dtype == FR_B200_T_F16) OP_CU(launch_ssm_seq<__half>(a, t, st));
     else if (dtype == FR_B200_T_BF16) OP_CU(launch_ssm_seq<__nv_bfloat16>(a, t, st));
     else OP_CU(launch_ssm_seq<float>(a, t, st));
@@ -608,7 +620,7 @@ int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, c
                      int N, int groups, float *state, int64_t state_stride, int n_slots, const int32_t *from, const int32_t *to, void *out,
                      int64_t ldo, int device, void *stream) {
   OP_TRY
-  SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, nullptr, ldx, lddt, ldb, ldc, ldz, ldo, state_stride, D, N, groups, dt_softplus != 0, 0, 0, 0};
+  SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, nullptr, ldx, lddt, ldb, ldc, ldz, ldo, state_stride, D, N, groups, dt_softplus != 0, 0, 0};
   int rc;
   if ((rc = ssm_check(a, dtype, n, n_slots)) || (rc = check_slots(n, state, n_slots, from, to))) return rc;
   a.vec = aligned(state, 16) && aligned(A, 16) && state_stride % 4 == 0 && N % 4 == 0;

@@ -16,65 +16,71 @@ struct SsmArgs {
   long long ldx, lddt, ldb, ldc, ldz, ldo, state_stride;   // elements
   int d, n, groups, softplus, vec;                         // vec: x, dt, z and out can be taken eight channels at a time
   int shift;                                               // pieces of 2^shift rows; 0: sequences whole
-  int wide;                                                // many states a thread: enough channels and sequences for all SMs
 };
 template <typename T> cudaError_t launch_ssm_seq(const SsmArgs &a, const SeqTable &t, cudaStream_t st);
 
 #ifdef FRB_SSM_KERNELS
 
-// A CTA walks its channels along the rows of a piece, SSM_ROWS at a time.  Half of its warps hold the states, a thread NS of one channel, L lanes a
-// channel; the others put down what these need of the next rows (time steps and their products with x, once per row and channel; B and
-// C) and finish the rows before (skip, gate, rounding, store), over two buffers and named barriers.
+// A CTA walks 128 / L channels along the rows of a piece, SSM_ROWS at a time, with three kinds of warps, each at a tile of its own:
+//   four hold the states, a lane NS of one channel, L lanes a channel;
+//   two bring the next rows in (copies two tiles ahead) and put down what the states need of them: time steps and their products with x, once
+//   per row and channel, B and C in fp32;
+//   two finish the rows behind: skip, gate, rounding, store.
+// (One warp that does all of it took four times as long for a row of its own: its chains of dependent instructions follow one another.)
+// Everything lies in shared memory along the rows: a lane takes four rows of a state with loads of 16 bytes, packed products of neighbouring rows and
+// one multiply-add a row.  The sums over a channel's lanes are taken L rows at a time, so that every lane ends with one row's (L - 1
+// shuffles for L rows).
+// What bounds it: with work for all SMs the words that lanes load from shared memory, 2 L + 32 a row of 32 channels (16 states), next
+// to 40 clocks of exponentials; alone, a warp's own latency, 42 clocks a row with one state a lane, 65 with two, 85 with four.
 //   SSM_WHOLE: the piece is the sequence      SSM_ENDS: the piece's state from zero, and the sum of its time steps
 //   SSM_PIECE: the piece from the state that the pieces before it leave
-// The sums over a channel's lanes are taken L rows at a time, so that every lane ends with one row's (L - 1 shuffles for L rows).
-// NS = 16 ("wide"): 58 instructions for 16 exponentials of 32 channels, which take the exponential unit 128 clocks; NS = 4, L = 4 has four times
-// the warps for a sequence alone, whose rows are a chain.
-constexpr int SSM_ROWS = 32;
+constexpr int SSM_ROWS = 32, SSM_STATES = 128, SSM_IN = 64, SSM_OUT = 64, SSM_THREADS = SSM_STATES + SSM_IN + SSM_OUT, SSM_RING = 4;
+constexpr int SSM_LD = SSM_ROWS + 4;   // 16 bytes more than the rows: eight lanes' loads meet in no bank
 enum { SSM_WHOLE = 0, SSM_ENDS = 1, SSM_PIECE = 2 };
-template <int NS, int L>
+template <typename T, int NS, int L>
 struct SsmTile {
-  static constexpr bool WIDE = L == 1 || NS >= 16;
-  static constexpr int THREADS = WIDE ? 64 : 128;             // of each half
-  static constexpr int CH = THREADS / L, NP = NS * L, YS = CH + 8;
-  static constexpr int EPT = CH >= 8 ? (CH * SSM_ROWS / THREADS < 8 ? CH * SSM_ROWS / THREADS : 8) : CH, TPR = CH / EPT;   // channels a thread puts down, threads a row
-  static constexpr int RPP = THREADS / TPR, PASSES = SSM_ROWS / RPP;   // rows put down at a time
-  float2 du[2][SSM_ROWS][CH];              // {delta, delta x}, where du_at says
-  float b[2][SSM_ROWS][NP], c[2][SSM_ROWS][NP];
+  static constexpr int CH = SSM_STATES / L, NP = NS * L, YS = CH + 8;   // (YS: L rows of 32 / L channels in 32 banks)
+  T in[SSM_RING][3][SSM_ROWS][CH + 16 / sizeof(T)];   // x, dt, z
+  float delta[2][CH][SSM_LD], u[2][CH][SSM_LD];      // time steps, times x
+  float b[2][NP][SSM_LD], c[2][NP][SSM_LD];          // state n where bc_at says: the states that the lanes read at a time lie side by side
+  static __device__ __forceinline__ int bc_at(int n) { return n % NS * L + n / NS; }
   float y[2][SSM_ROWS][YS];
 };
-// place of a channel in its row: turned, so that the threads that write eight channels each do not meet in a bank
-__device__ __forceinline__ int du_at(int ch, int row) { return (ch & ~7) | ((ch + 2 * (ch >> 3) + (row & 1)) & 7); }
-enum { SSM_BAR_FULL = 1, SSM_BAR_DONE = 3, SSM_BAR_SUM = 5 };
+// named barriers, two of each: rows put down; states done with them; rows finished (their buffers are free)
+enum { SSM_BAR_FULL = 1, SSM_BAR_DONE = 3, SSM_BAR_FREE = 5, SSM_BAR_IN = 7 };
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+template <int ID, int N> __device__ __forceinline__ void pair_sync(int which) { if (which) asm volatile("bar.sync %0, %1;" ::"n"(ID + 1), "n"(N) : "memory"); else asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+template <int ID, int N> __device__ __forceinline__ void pair_arrive(int which) { if (which) asm volatile("bar.arrive %0, %1;" ::"n"(ID + 1), "n"(N) : "memory"); else asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+__device__ __forceinline__ void copy_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ float2 two_of(unsigned long long v) {
   float2 r;
   unpack_f2(v, r.x, r.y);
   return r;
 }
 
-template <typename T, int NS, int L, int MODE, bool VEC>
-__global__ void __launch_bounds__(2 * SsmTile<NS, L>::THREADS, SsmTile<NS, L>::WIDE ? 4 : 2)
-ssm_seq_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
-  using Tile = SsmTile<NS, L>;
-  constexpr int CH = Tile::CH, NP = Tile::NP, HALF = Tile::THREADS, PAIRS = NS / 2;
+template <typename T, int NS, int L, int CTAS, int MODE, bool VEC>
+__global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
+  using Tile = SsmTile<T, NS, L>;
+  constexpr int CH = Tile::CH, NP = Tile::NP;
+  constexpr int FULL_N = SSM_STATES + SSM_IN, DONE_N = SSM_STATES + SSM_OUT, FREE_N = SSM_IN + (MODE == SSM_ENDS ? SSM_STATES : SSM_OUT);
   extern __shared__ __align__(16) uint8_t ssm_smem[];
   Tile &sm = *reinterpret_cast<Tile *>(ssm_smem);
   int s, piece = 0;
   long long row, end;
   if (MODE == SSM_WHOLE) {
-    s = blockIdx.y; row = tab.first[s]; end = tab.first[s + 1];
+    s = blockIdx.y; row = tab.first[s]; end = tab.end[s];
   } else {
-    s = seq_of(tab, blockIdx.y, a.shift);
-    piece = blockIdx.y - seq_key(tab, s, a.shift);
+    s = seq_of(tab, blockIdx.y);
+    piece = blockIdx.y - tab.key[s];
     row = tab.first[s] + ((long long)piece << a.shift);
-    end = tab.first[s + 1];
+    end = tab.end[s];
     if (end - row > (1ll << a.shift)) end = row + (1ll << a.shift);
   }
   pdl_wait();
-  pdl_trigger();
   if (MODE != SSM_WHOLE && piece > 0 && row >= end) return;
-  const bool last = MODE == SSM_WHOLE || end == tab.first[s + 1];
+  const bool last = MODE == SSM_WHOLE || end == tab.end[s];
   if (MODE == SSM_ENDS && last) return;   // nobody follows the last piece
   // the channels of a CTA are of one group
   const int per_group = a.d / a.groups, ctas = (per_group + CH - 1) / CH, group = blockIdx.x / ctas;
@@ -83,271 +89,263 @@ ssm_seq_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
   float *work = MODE != SSM_WHOLE ? a.work + (size_t)blockIdx.y * (dn + a.d) : nullptr;
   const int tiles = (int)((end - row + SSM_ROWS - 1) / SSM_ROWS), full = (int)((end - row) / SSM_ROWS);
 
-  if (threadIdx.x < HALF) {
+  if (threadIdx.x < SSM_STATES) {
     // ---- the states ----
     const int tid = threadIdx.x, lane = tid % L, ch_in = tid / L, ch = ch0 + ch_in, n0 = lane * NS;
     const bool live = ch < ch_end;
     const float *slot = nullptr;
     if (MODE == SSM_WHOLE) { if (tab.from[s] >= 0) slot = a.state + tab.from[s] * a.state_stride; }
     else if (MODE == SSM_PIECE) slot = work;
-    unsigned long long A2[PAIRS], h[PAIRS];
+    float h[NS];
+    unsigned long long A2[NS];
 #pragma unroll
-    for (int i = 0; i < NS; i += 2) {
-      float av[2], hv[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const bool there = live && n0 + i + q < a.n;
-        av[q] = there ? a.A[(size_t)ch * a.n + n0 + i + q] * LOG2E : 0.f;
-        hv[q] = there && slot ? slot[(size_t)ch * a.n + n0 + i + q] : 0.f;
-      }
-      A2[i / 2] = pack_f2(av[0], av[1]);
-      h[i / 2] = pack_f2(hv[0], hv[1]);
+    for (int i = 0; i < NS; ++i) {
+      const bool there = live && n0 + i < a.n;
+      const float av = there ? a.A[(size_t)ch * a.n + n0 + i] * LOG2E : 0.f;
+      A2[i] = pack_f2(av, av);
+      h[i] = there && slot ? slot[(size_t)ch * a.n + n0 + i] : 0.f;
     }
-    const int at[2] = {du_at(ch_in, 0), du_at(ch_in, 1)};
-    auto pair_at = [](const float *p) { return *reinterpret_cast<const unsigned long long *>(p); };
-    // one row whole; its part of y
-    auto one_row = [&](int buf, int t, int odd) {
-      const float2 du = sm.du[buf][t][at[odd]];
-      const unsigned long long dd = pack_f2(du.x, du.x), uu = pack_f2(du.y, du.y);
-      unsigned long long y[2] = {0, 0};
+    // rows t .. t + 3; left: rows there are (those behind the end have no say, whatever exp makes of 0 x A)
+    auto four_rows = [&](auto whole, int buf, int t, int left, float *p) {
+      const ulonglong2 d4 = *reinterpret_cast<const ulonglong2 *>(&sm.delta[buf][ch_in][t]), u4 = *reinterpret_cast<const ulonglong2 *>(&sm.u[buf][ch_in][t]);
+      unsigned long long y01 = 0, y23 = 0;
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        const float2 e = two_of(mul_f2(dd, A2[i]));
-        h[i] = fma_f2(pack_f2(ex2(e.x), ex2(e.y)), h[i], mul_f2(uu, pair_at(&sm.b[buf][t][n0 + 2 * i])));
+      for (int i = 0; i < NS; ++i) {
+        const ulonglong2 b4 = *reinterpret_cast<const ulonglong2 *>(&sm.b[buf][i * L + lane][t]);
+        const float2 e01 = two_of(mul_f2(d4.x, A2[i])), e23 = two_of(mul_f2(d4.y, A2[i]));
+        const float2 w01 = two_of(mul_f2(u4.x, b4.x)), w23 = two_of(mul_f2(u4.y, b4.y));
+        const float e[4] = {e01.x, e01.y, e23.x, e23.y}, w[4] = {w01.x, w01.y, w23.x, w23.y};
+        float hs[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float next = fmaf(ex2(e[q]), h[i], w[q]);
+          h[i] = decltype(whole)::value || t + q < left ? next : h[i];
+          hs[q] = h[i];
+        }
         if (MODE != SSM_ENDS) {
-          const unsigned long long c = pair_at(&sm.c[buf][t][n0 + 2 * i]);
-          y[i & 1] = i > 1 ? fma_f2(h[i], c, y[i & 1]) : mul_f2(h[i], c);
+          const ulonglong2 c4 = *reinterpret_cast<const ulonglong2 *>(&sm.c[buf][i * L + lane][t]);
+          y01 = i ? fma_f2(pack_f2(hs[0], hs[1]), c4.x, y01) : mul_f2(pack_f2(hs[0], hs[1]), c4.x);
+          y23 = i ? fma_f2(pack_f2(hs[2], hs[3]), c4.y, y23) : mul_f2(pack_f2(hs[2], hs[3]), c4.y);
         }
       }
-      const float2 y0 = two_of(y[0]), y1 = two_of(y[1]);
-      return PAIRS > 1 ? (y0.x + y0.y) + (y1.x + y1.y) : y0.x + y0.y;
+      const float2 p01 = two_of(y01), p23 = two_of(y23);
+      p[0] = p01.x; p[1] = p01.y; p[2] = p23.x; p[3] = p23.y;
     };
-    // L rows' parts -> every lane the sum of one of them
-    auto join = [&](float (&p)[L]) {
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int q = 0; q < o; ++q) {
-          const float send = up ? p[q] : p[q + o], keep = up ? p[q + o] : p[q];
-          p[q] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-      }
-      return p[0];
-    };
-    if constexpr (Tile::WIDE) {
-      for (int k = 0; k < full; ++k) {
-        const int buf = k & 1;
-        bar_sync(SSM_BAR_FULL + buf, 2 * HALF);
-        constexpr int STEP = L > 2 ? L : 2;
+    auto tile = [&](auto whole, int buf, int left) {
+      constexpr int STEP = L > 8 ? L : 8;
 #pragma unroll 1
-        for (int t0 = 0; t0 < SSM_ROWS; t0 += STEP) {
-          float y[STEP];
+      for (int t0 = 0; t0 < (decltype(whole)::value ? SSM_ROWS : left); t0 += STEP) {
+        float p[STEP];
 #pragma unroll
-          for (int q = 0; q < STEP; ++q) y[q] = one_row(buf, t0 + q, q & 1);
-          if (MODE != SSM_ENDS)
+        for (int r = 0; r < STEP; r += 4) four_rows(whole, buf, t0 + r, left, p + r);
+        if (MODE != SSM_ENDS)
+          // L rows' parts -> every lane the sum of one of them
 #pragma unroll
-            for (int q = 0; q < STEP; q += L) {
-              float p[L];
+          for (int g = 0; g < STEP; g += L) {
 #pragma unroll
-              for (int r = 0; r < L; ++r) p[r] = y[q + r];
-              sm.y[buf][t0 + q + lane][ch_in] = join(p);
-            }
-        }
-        bar_arrive(SSM_BAR_DONE + buf, 2 * HALF);
-      }
-    } else {
-      // G rows at a time: their decays and what they add are made one turn ahead, so that the exponentials of one turn run beside the chain
-      // and the shuffles of the other (in one turn, a row took 107 clocks, its exponentials 32)
-      constexpr int G = NS >= 8 ? 2 : 4, STEP = L > 2 * G ? L : 2 * G, TURNS = STEP / G;
-      struct Turn { unsigned long long decay[G][PAIRS], add[G][PAIRS]; } turn[2];
-      auto prepare = [&](Turn &r, int buf, int t) {
+            for (int o = L / 2; o > 0; o >>= 1) {
+              const bool up = lane & o;
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-          const float2 du = sm.du[buf][t + q][at[q & 1]];
-          const unsigned long long dd = pack_f2(du.x, du.x), uu = pack_f2(du.y, du.y);
-#pragma unroll
-          for (int i = 0; i < PAIRS; ++i) {
-            const float2 e = two_of(mul_f2(dd, A2[i]));
-            r.decay[q][i] = pack_f2(ex2(e.x), ex2(e.y));
-            r.add[q][i] = mul_f2(uu, pair_at(&sm.b[buf][t + q][n0 + 2 * i]));
-          }
-        }
-      };
-      if (full > 0) {
-        bar_sync(SSM_BAR_FULL, 2 * HALF);
-        prepare(turn[0], 0, 0);
-      }
-      for (int k = 0; k < full; ++k) {
-        const int buf = k & 1;
-#pragma unroll 1
-        for (int t0 = 0; t0 < SSM_ROWS; t0 += STEP) {
-          float p[L];
-#pragma unroll
-          for (int u = 0; u < TURNS; ++u) {
-            if (u + 1 < TURNS || t0 + STEP < SSM_ROWS) prepare(turn[(u + 1) & 1], buf, t0 + (u + 1) * G);
-            else if (k + 1 < full) {
-              bar_sync(SSM_BAR_FULL + (buf ^ 1), 2 * HALF);
-              prepare(turn[0], buf ^ 1, 0);
-            }
-#pragma unroll
-            for (int q = 0; q < G; ++q) {
-              unsigned long long y = 0;
-#pragma unroll
-              for (int i = 0; i < PAIRS; ++i) {
-                h[i] = fma_f2(turn[u & 1].decay[q][i], h[i], turn[u & 1].add[q][i]);
-                if (MODE != SSM_ENDS) {
-                  const unsigned long long c = pair_at(&sm.c[buf][t0 + u * G + q][n0 + 2 * i]);
-                  y = i ? fma_f2(h[i], c, y) : mul_f2(h[i], c);
-                }
+              for (int q = 0; q < o; ++q) {
+                const float send = up ? p[g + q] : p[g + q + o], keep = up ? p[g + q + o] : p[g + q];
+                p[g + q] = keep + __shfl_xor_sync(0xffffffffu, send, o);
               }
-              const float2 yy = two_of(y);
-              p[(u * G + q) % L] = yy.x + yy.y;
             }
-            if (MODE != SSM_ENDS && (u + 1) * G % L == 0) sm.y[buf][t0 + (u + 1) * G - L + lane][ch_in] = join(p);
+            sm.y[buf][t0 + g + lane][ch_in] = p[g];
           }
-        }
-        bar_arrive(SSM_BAR_DONE + buf, 2 * HALF);
       }
-    }
-    if (full < tiles) {   // the rows that are left; those behind the end have no say, whatever exp makes of 0 x A
-      const int buf = full & 1, left = (int)(end - row) - full * SSM_ROWS;
-      bar_sync(SSM_BAR_FULL + buf, 2 * HALF);
-      for (int t0 = 0; t0 < left; t0 += L) {
-        float p[L];
-#pragma unroll
-        for (int q = 0; q < L; ++q) {
-          p[q] = 0.f;
-          if (t0 + q < left) p[q] = one_row(buf, t0 + q, (t0 + q) & 1);
-        }
-        if (MODE != SSM_ENDS) sm.y[buf][t0 + lane][ch_in] = join(p);
-      }
-      bar_arrive(SSM_BAR_DONE + buf, 2 * HALF);
+    };
+    for (int k = 0; k < tiles; ++k) {
+      const int buf = k & 1;
+      pair_sync<SSM_BAR_FULL, FULL_N>(buf);
+      if (k < full) tile(std::true_type{}, buf, SSM_ROWS);
+      else tile(std::false_type{}, buf, (int)(end - row) - full * SSM_ROWS);
+      if (MODE == SSM_ENDS) pair_arrive<SSM_BAR_FREE, FREE_N>(buf);
+      else pair_arrive<SSM_BAR_DONE, DONE_N>(buf);
     }
     float *to = nullptr;
     if (MODE == SSM_ENDS) to = work;
     else if (last && tab.to[s] >= 0) to = a.state + tab.to[s] * a.state_stride;
     if (to)
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const float2 hh = two_of(h[i / 2]);
-        if (live && n0 + i < a.n) to[(size_t)ch * a.n + n0 + i] = i & 1 ? hh.y : hh.x;
-      }
+      for (int i = 0; i < NS; ++i)
+        if (live && n0 + i < a.n) to[(size_t)ch * a.n + n0 + i] = h[i];
     return;
   }
 
-  // ---- rows in and out: EPT channels of PASSES rows a thread ----
-  constexpr int EPT = Tile::EPT, TPR = Tile::TPR, RPP = Tile::RPP, PASSES = Tile::PASSES;
-  const int tid = threadIdx.x - HALF, lr = tid / TPR, lc = (tid % TPR) * EPT, gc = ch0 + lc;
-  const int ln = min(max(ch_end - gc, 0), EPT);
-  const int ga = ln > 0 ? gc : ch0, la = ln > 0 ? ln : 1;   // what is loaded by threads without channels: something that is there
-  float bias[EPT], skip[EPT], dsum[EPT];
+  const int ch_left = ch_end - ch0;   // channels of the tile that there are
+  if (threadIdx.x < SSM_STATES + SSM_IN) {
+    // ---- rows in ----
+    // a thread's places in a tile: a warp takes eight rows of eight channels at a time (four lanes, two channels each), in which neither its loads
+    // along the channels nor its stores along the rows meet in a bank
+    const int tid = threadIdx.x - SSM_STATES, sub = tid & 3;
+    constexpr int BLOCKS = CH / 8, EACH = BLOCKS * 2, ARRAYS = MODE == SSM_ENDS ? 2 : 3;   // (two warps, 16 rows each)
+    auto row_of = [&](int i) { return tid / 32 * 16 + i / BLOCKS * 8 + (tid & 31) / 4; };
+    auto ch_of = [&](int i) { return i % BLOCKS * 8 + sub * 2; };
+    float bias[BLOCKS][2], dsum[BLOCKS][2];
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    bias[i] = i < ln && a.dt_bias ? a.dt_bias[gc + i] : 0.f;
-    skip[i] = i < ln && a.D && MODE != SSM_ENDS ? a.D[gc + i] : 0.f;
-    dsum[i] = 0.f;
+    for (int g = 0; g < BLOCKS; ++g)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        bias[g][e] = a.dt_bias && ch_of(g) + e < ch_left ? a.dt_bias[ch0 + ch_of(g) + e] : 0.f;
+        dsum[g][e] = 0.f;
+      }
+    const T *src[3] = {reinterpret_cast<const T *>(a.x) + ch0, reinterpret_cast<const T *>(a.dt) + ch0, reinterpret_cast<const T *>(a.z ? a.z : a.x) + ch0};
+    const long long ld[3] = {a.ldx, a.lddt, a.z ? a.ldz : a.ldx};
+    // Rows and channels past the end repeat the last (and count for nothing): a load that is made or not is waited for where its ways meet.
+    constexpr int UNIT = 16 / (int)sizeof(T), ROW_UNITS = CH / UNIT, COPIES = SSM_ROWS * ROW_UNITS, PER = (COPIES + SSM_IN - 1) / SSM_IN;
+    constexpr int SINGLE = SSM_ROWS * CH / SSM_IN;
+    T hold[VEC ? 1 : 3 * SINGLE];
+    auto ask = [&](int k) {   // tile k: copies into its place in the ring, or (not VEC) elements into registers
+      const long long t0 = row + (long long)k * SSM_ROWS;
+      const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
+#pragma unroll
+      for (int arr = 0; arr < ARRAYS; ++arr) {
+        if constexpr (VEC) {
+#pragma unroll
+          for (int q = 0; q < PER; ++q) {
+            const int e = tid + q * SSM_IN, r = e / ROW_UNITS, c = e % ROW_UNITS * UNIT;
+            if (e < COPIES) copy_async16(&sm.in[k % SSM_RING][arr][r][c], src[arr] + (t0 + min(r, final_row)) * ld[arr] + min(c, (ch_left - 1) / UNIT * UNIT));
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < SINGLE; ++q) {
+            const int e = tid + q * SSM_IN;
+            hold[arr * SINGLE + q] = src[arr][(t0 + min(e / CH, final_row)) * ld[arr] + min(e % CH, ch_left - 1)];
+          }
+        }
+      }
+      if (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto keep = [&](int k) {
+      if constexpr (!VEC) {
+#pragma unroll
+        for (int arr = 0; arr < ARRAYS; ++arr)
+#pragma unroll
+          for (int q = 0; q < SINGLE; ++q) sm.in[k % SSM_RING][arr][(tid + q * SSM_IN) / CH][(tid + q * SSM_IN) % CH] = hold[arr * SINGLE + q];
+      }
+    };
+    // B and C: one column, every BROWS-th row (or all rows of several columns); columns past the last are 0
+    constexpr int BROWS = SSM_IN >= NP ? SSM_IN / NP : 1, BCOLS = SSM_IN >= NP ? 1 : NP / SSM_IN, BPT = SSM_ROWS / BROWS * BCOLS, BATCH = BPT < 16 ? BPT : 16;
+    const int bcol = tid % NP, brow = tid / NP;
+    const T *bp = reinterpret_cast<const T *>(a.B) + (long long)group * a.n, *cp = reinterpret_cast<const T *>(a.C) + (long long)group * a.n;
+    T bn[BATCH], cn[BATCH];
+    auto bc_ask = [&](int k, int q0) {
+      const long long t0 = row + (long long)k * SSM_ROWS;
+      const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
+      const T *b = bp + t0 * a.ldb, *c = cp + t0 * a.ldc;
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
+        const int r = min(brow + (q0 + q) / BCOLS * BROWS, final_row), col = min(bcol + (q0 + q) % BCOLS * SSM_IN, a.n - 1);
+        bn[q] = b[r * a.ldb + col];
+        if (MODE != SSM_ENDS) cn[q] = c[r * a.ldc + col];
+      }
+    };
+    auto bc_put = [&](int buf, int q0) {
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
+        const int r = brow + (q0 + q) / BCOLS * BROWS, col = bcol + (q0 + q) % BCOLS * SSM_IN;
+        sm.b[buf][Tile::bc_at(col)][r] = col < a.n ? to_f(bn[q]) : 0.f;
+        if (MODE != SSM_ENDS) sm.c[buf][Tile::bc_at(col)][r] = col < a.n ? to_f(cn[q]) : 0.f;
+      }
+    };
+    if (tiles > 0) {
+      ask(0);
+      if (VEC) ask(1);   // (past the end too: the last row again)
+      bc_ask(0, 0);
+    }
+    for (int k = 0; k < tiles; ++k) {
+      const int buf = k & 1;
+      if (k >= 2) pair_sync<SSM_BAR_FREE, FREE_N>(buf);   // tile k - 2 is finished
+      if (VEC) {
+        ask(k + 2);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      } else {
+        keep(k);
+        ask(k + 1);
+      }
+      pair_sync<SSM_BAR_IN, SSM_IN>(0);   // everybody's part of tile k is there
+      const long long t0 = row + (long long)k * SSM_ROWS;
+Pack<T, 2> x[EACH], dt[EACH];   // (all of them ahead of the first store, which a load would have to stay behind)
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int r = row_of(i), c = ch_of(i);
+        x[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][0][r][c]);
+        dt[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][1][r][c]);
+      }
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int r = row_of(i), c = ch_of(i);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = to_f(dt[i].v[e]) + bias[i % BLOCKS][e];
+          if (a.softplus) v = softplus(v);
+          if (MODE == SSM_ENDS && t0 + r < end) dsum[i % BLOCKS][e] += v;
+          sm.delta[buf][c + e][r] = v;
+          sm.u[buf][c + e][r] = v * to_f(x[i].v[e]);
+        }
+      }
+      bc_put(buf, 0);
+      for (int q0 = BATCH; q0 < BPT; q0 += BATCH) { bc_ask(k, q0); bc_put(buf, q0); }
+      bc_ask(k + 1, 0);
+      pair_arrive<SSM_BAR_FULL, FULL_N>(buf);
+    }
+    if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (tiles > 1) pair_sync<SSM_BAR_FREE, FREE_N>(tiles & 1);
+    if (tiles > 0) pair_sync<SSM_BAR_FREE, FREE_N>((tiles - 1) & 1);
+    if (MODE == SSM_ENDS) {
+      // the sum of a channel's time steps, over the rows' threads in a fixed order (the buffers are free)
+#pragma unroll
+      for (int g = 0; g < BLOCKS; ++g)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sm.y[0][tid / 4][ch_of(g) + e] = dsum[g][e];
+      pair_sync<SSM_BAR_IN, SSM_IN>(0);
+      for (int c = tid; c < CH && c < ch_left; c += SSM_IN) {
+        float v = 0.f;
+        for (int r = 0; r < SSM_IN / 4; ++r) v += sm.y[0][r][c];
+        work[dn + ch0 + c] = v;
+      }
+    }
+    return;
   }
-  const T *xp = reinterpret_cast<const T *>(a.x) + ga, *dtp = reinterpret_cast<const T *>(a.dt) + ga;
-  const T *zp = a.z ? reinterpret_cast<const T *>(a.z) + ga : xp;
-  const long long ldz = a.z ? a.ldz : a.ldx;
-  T *op = reinterpret_cast<T *>(a.out) + gc;
-  // B and C: one column, every (HALF / NP)-th row a thread (or every column of (NP / HALF) ones)
-  constexpr int BROWS = HALF >= NP ? HALF / NP : 1, BCOLS = HALF >= NP ? 1 : NP / HALF, BPT = SSM_ROWS / BROWS * BCOLS;
-  constexpr bool BC_AHEAD = BPT <= 8;   // more of them are fetched when they are put down: there is more work to a row then
-  const int bcol = tid % NP, brow = tid / NP;
-  const T *bp = reinterpret_cast<const T *>(a.B) + (long long)group * a.n, *cp = reinterpret_cast<const T *>(a.C) + (long long)group * a.n;
 
-  // rows and columns past the end repeat the last (and count for nothing): a load that is made or not is waited for
-  Pack<T, EPT> xa[PASSES], da[PASSES];
-  T bn[BC_AHEAD ? BPT : 1], cn[BC_AHEAD ? BPT : 1];
-  auto fetch = [&](long long r0) {
-    const int final_row = (int)min(end - 1 - r0, (long long)SSM_ROWS - 1);
+  // ---- rows out ----
+  if constexpr (MODE != SSM_ENDS) {
+    // a thread's places: two channels of every STRIDE-th row
+    constexpr int CP = CH / 2;   // (up to 64 threads)
+    const int tid = threadIdx.x - SSM_STATES - SSM_IN, cc = tid % CP * 2, r0 = tid / CP;
+    constexpr int STRIDE = SSM_OUT / CP, EACH = SSM_ROWS / STRIDE;
+    float skip[2];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const long long r = r0 + min(lr + i * RPP, final_row);
-      xa[i] = load_pack<T, EPT, VEC>(xp + r * a.ldx, la);
-      da[i] = load_pack<T, EPT, VEC>(dtp + r * a.lddt, la);
-    }
-    if (BC_AHEAD)
+    for (int i = 0; i < 2; ++i) skip[i] = a.D && cc + i < ch_left ? a.D[ch0 + cc + i] : 0.f;
+    T *op = reinterpret_cast<T *>(a.out) + ch0 + cc;
+    for (int k = 0; k < tiles; ++k) {
+      const int buf = k & 1;
+      const long long t0 = row + (long long)k * SSM_ROWS;
+      pair_sync<SSM_BAR_DONE, DONE_N>(buf);
+Pack<T, 2> x[EACH], z[EACH];
+      float2 yv[EACH];
 #pragma unroll
-      for (int q = 0; q < BPT; ++q) {
-        const int r = min(brow + q / BCOLS * BROWS, final_row), col = min(bcol + q % BCOLS * HALF, a.n - 1);
-        bn[q] = bp[r0 * a.ldb + col + r * a.ldb];
-        if (MODE != SSM_ENDS) cn[q] = cp[r0 * a.ldc + col + r * a.ldc];
+      for (int i = 0; i < EACH; ++i) {
+        const int r = r0 + i * STRIDE;
+        x[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][0][r][cc]);
+        z[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][2][r][cc]);
+        yv[i] = *reinterpret_cast<const float2 *>(&sm.y[buf][r][cc]);
       }
-  };
-  auto put_down = [&](long long r0, int buf) {
-    const int final_row = (int)min(end - 1 - r0, (long long)SSM_ROWS - 1);
+      pair_arrive<SSM_BAR_FREE, FREE_N>(buf);
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int r = lr + i * RPP;
+      for (int i = 0; i < EACH; ++i) {
+        const int r = r0 + i * STRIDE;
+        float y[2] = {yv[i].x, yv[i].y};
+        Pack<T, 2> o;
 #pragma unroll
-      for (int e = 0; e < EPT; ++e) {
-        float v = to_f(da[i].v[e]) + bias[e];
-        if (a.softplus) v = softplus(v);
-        sm.du[buf][r][du_at(lc + e, r)] = make_float2(v, v * to_f(xa[i].v[e]));
-        if (MODE == SSM_ENDS && r <= final_row) dsum[e] += v;
+        for (int e = 0; e < 2; ++e) {
+          y[e] = fmaf(skip[e], to_f(x[i].v[e]), y[e]);
+          if (a.z) y[e] *= silu(to_f(z[i].v[e]));
+          o.v[e] = from_f<T>(y[e]);
+        }
+        if (t0 + r < end && cc < ch_left) store_pack<T, 2, VEC>(op + (t0 + r) * a.ldo, o, ch_left - cc);
       }
-    }
-#pragma unroll 8
-    for (int q = 0; q < BPT; ++q) {
-      const int r = brow + q / BCOLS * BROWS, col = bcol + q % BCOLS * HALF;
-      if (!BC_AHEAD) {
-        const long long rr = r0 + min(r, final_row);
-        bn[0] = bp[rr * a.ldb + min(col, a.n - 1)];
-        if (MODE != SSM_ENDS) cn[0] = cp[rr * a.ldc + min(col, a.n - 1)];
-      }
-      sm.b[buf][r][col] = col < a.n ? to_f(bn[BC_AHEAD ? q : 0]) : 0.f;
-      if (MODE != SSM_ENDS) sm.c[buf][r][col] = col < a.n ? to_f(cn[BC_AHEAD ? q : 0]) : 0.f;
-    }
-  };
-  if (tiles > 0) {
-    fetch(row);
-    put_down(row, 0);
-    bar_arrive(SSM_BAR_FULL, 2 * HALF);
-    if (tiles > 1) fetch(row + SSM_ROWS);
-  }
-  for (int k = 0; k < tiles; ++k, row += SSM_ROWS) {
-    const int buf = k & 1, final_row = (int)min(end - 1 - row, (long long)SSM_ROWS - 1);
-    if (k + 1 < tiles) {   // (the other buffer: its rows were finished in the turn before)
-      put_down(row + SSM_ROWS, buf ^ 1);
-      bar_arrive(SSM_BAR_FULL + (buf ^ 1), 2 * HALF);
-      if (k + 2 < tiles) fetch(row + 2 * SSM_ROWS);
-    }
-    if constexpr (MODE == SSM_ENDS) bar_sync(SSM_BAR_DONE + buf, 2 * HALF);
-    else {
-    Pack<T, EPT> xe[PASSES], ze[PASSES];   // (x once more, out of the L2)
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const long long r = row + min(lr + i * RPP, final_row);
-      xe[i] = load_pack<T, EPT, VEC>(xp + r * a.ldx, la);
-      ze[i] = load_pack<T, EPT, VEC>(zp + r * ldz, la);
-    }
-    bar_sync(SSM_BAR_DONE + buf, 2 * HALF);
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int r = lr + i * RPP;
-      Pack<T, EPT> o;
-#pragma unroll
-      for (int e = 0; e < EPT; ++e) {
-        float y = fmaf(skip[e], to_f(xe[i].v[e]), sm.y[buf][r][lc + e]);
-        if (a.z) y *= silu(to_f(ze[i].v[e]));
-        o.v[e] = from_f<T>(y);
-      }
-      if (r <= final_row && ln > 0) store_pack<T, EPT, VEC>(op + (row + r) * a.ldo, o, ln);
-    }
-    }
-  }
-  if (MODE == SSM_ENDS) {
-    // the sum of a channel's time steps, over the rows' threads in a fixed order
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) sm.y[0][lr][lc + e] = dsum[e];
-    bar_sync(SSM_BAR_SUM, HALF);
-    if (tid < CH && ch0 + tid < ch_end) {
-      float v = 0.f;
-      for (int r = 0; r < RPP; ++r) v += sm.y[0][r][tid];
-      work[dn + ch0 + tid] = v;
     }
   }
 }
@@ -360,9 +358,9 @@ static __global__ void __launch_bounds__(256) ssm_join_kernel(const SsmArgs a, c
   pdl_wait();
   pdl_trigger();
   if (e >= (long long)dn) return;
-  const long long len = tab.first[s + 1] - tab.first[s];
+  const long long len = tab.end[s] - tab.first[s];
   const int pieces = len > 0 ? (int)((len + (1ll << a.shift) - 1) >> a.shift) : 1, ch = e / a.n;
-  float *w = a.work + (size_t)seq_key(tab, s, a.shift) * (dn + a.d);
+  float *w = a.work + (size_t)tab.key[s] * (dn + a.d);
   const float A2 = a.A[e] * LOG2E;
   float S = tab.from[s] >= 0 ? a.state[tab.from[s] * a.state_stride + e] : 0.f;
   constexpr int AHEAD = 8;   // pieces asked for at a time (past the last: the last but one again)
@@ -383,31 +381,54 @@ static __global__ void __launch_bounds__(256) ssm_join_kernel(const SsmArgs a, c
   }
 }
 
-template <typename T, int NS, int L, int MODE, bool VEC>
+template <typename T, int NS, int L, int CTAS, int MODE, bool VEC>
 cudaError_t ssm_seq_mode(const SsmArgs &a, const SeqTable &t, int items, cudaStream_t st) {
-  using Tile = SsmTile<NS, L>;
+  using Tile = SsmTile<T, NS, L>;
   static thread_local uint64_t told = 0;
-  cudaError_t e = allow_smem(ssm_seq_kernel<T, NS, L, MODE, VEC>, (int)sizeof(Tile), told);
+  cudaError_t e = allow_smem(ssm_seq_kernel<T, NS, L, CTAS, MODE, VEC>, (int)sizeof(Tile), told);
   if (e != cudaSuccess) return e;
   const dim3 grid((a.d / a.groups + Tile::CH - 1) / Tile::CH * a.groups, items);
-  return op_launch(ssm_seq_kernel<T, NS, L, MODE, VEC>, grid, 2 * Tile::THREADS, sizeof(Tile), st, 1, a, t);
+  return op_launch(ssm_seq_kernel<T, NS, L, CTAS, MODE, VEC>, grid, SSM_THREADS, sizeof(Tile), st, 1, a, t);
 }
-// NW states a thread and LW lanes a channel where there is work for all SMs (whole sequences, or pieces of them); else NS and L
-template <typename T, int NW, int LW, int NS, int L, bool VEC>
-cudaError_t ssm_seq_launch(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {
-  if (!a.shift) return a.wide ? ssm_seq_mode<T, NW, LW, SSM_WHOLE, VEC>(a, t, t.n, st) : ssm_seq_mode<T, NS, L, SSM_WHOLE, VEC>(a, t, t.n, st);
-  const int items = seq_items(t, a.shift);
-  cudaError_t e = ssm_seq_mode<T, NW, LW, SSM_ENDS, VEC>(a, t, items, st);
+template <typename T, int NS, int L, bool VEC>
+cudaError_t ssm_seq_split(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {
+  const int items = t.key[t.n];
+  cudaError_t e = ssm_seq_mode<T, NS, L, 2, SSM_ENDS, VEC>(a, t, items, st);
   if (e == cudaSuccess) e = op_launch(ssm_join_kernel, dim3((unsigned)(((size_t)a.d * a.n + 255) / 256), t.n), 256, 0, st, 1, a, t);
-  return e == cudaSuccess ? ssm_seq_mode<T, NW, LW, SSM_PIECE, VEC>(a, t, items, st) : e;
+  return e == cudaSuccess ? ssm_seq_mode<T, NS, L, 2, SSM_PIECE, VEC>(a, t, items, st) : e;
 }
+// States a lane.  Few channels and sequences: fewer states, more CTAs and the shorter chain, as long as every CTA has an SM (4096 rows of 768
+// channels with 16 states: 92 us with one a lane, 141 with two, 184 with four; of 1536: 136, 141, 184; of 2560: 219, 205, 185).  Many:
+// three CTAs an SM where their registers allow it (11 sequences of 5120 channels 118 us against 131; one of 4096 230 against 186).
 template <typename T, bool VEC>
 cudaError_t ssm_seq_any(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {
-  if (a.n <= 8) return ssm_seq_launch<T, 8, 1, 2, 4, VEC>(a, t, st);
-  if (a.n <= 16) return ssm_seq_launch<T, 16, 1, 4, 4, VEC>(a, t, st);
-  if (a.n <= 32) return ssm_seq_launch<T, 16, 2, 4, 8, VEC>(a, t, st);
-  if (a.n <= 64) return ssm_seq_launch<T, 16, 4, 8, 8, VEC>(a, t, st);
-  return ssm_seq_launch<T, 16, 8, 8, 16, VEC>(a, t, st);
+  auto ctas = [&](int ch) { return (long long)((a.d / a.groups + ch - 1) / ch) * a.groups * t.n; };
+  const int sms = device_sm_count();
+  if (a.n <= 8) {
+    if (a.shift) return ssm_seq_split<T, 2, 4, VEC>(a, t, st);
+    if (ctas(16) <= sms) return ssm_seq_mode<T, 1, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(32) <= 2 * sms) return ssm_seq_mode<T, 2, 4, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    return ssm_seq_mode<T, 2, 4, 3, SSM_WHOLE, VEC>(a, t, t.n, st);
+  }
+  if (a.n <= 16) {
+    if (a.shift) return ssm_seq_split<T, 4, 4, VEC>(a, t, st);
+    if (ctas(8) <= sms) return ssm_seq_mode<T, 1, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(16) <= sms) return ssm_seq_mode<T, 2, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(32) <= 2 * sms) return ssm_seq_mode<T, 4, 4, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    return ssm_seq_mode<T, 4, 4, 3, SSM_WHOLE, VEC>(a, t, t.n, st);
+  }
+  if (a.n <= 32) {
+    if (a.shift) return ssm_seq_split<T, 4, 8, VEC>(a, t, st);
+    if (ctas(8) <= sms) return ssm_seq_mode<T, 2, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    return ssm_seq_mode<T, 4, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+  }
+  if (a.n <= 64) {
+    if (a.shift) return ssm_seq_split<T, 8, 8, VEC>(a, t, st);
+    if (ctas(8) <= sms) return ssm_seq_mode<T, 4, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    return ssm_seq_mode<T, 8, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+  }
+  if (a.shift) return ssm_seq_split<T, 8, 16, VEC>(a, t, st);
+  return ssm_seq_mode<T, 8, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
 }
 template <typename T>
 cudaError_t launch_ssm_seq(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {

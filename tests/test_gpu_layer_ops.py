@@ -346,6 +346,23 @@ def test_ssm_seq(pkg, lengths, d, n, g, dtype):
         _check(p, new, enew, "state")
 
 
+@pytest.mark.parametrize("d,n,g,dtype", [(2056, 16, 1, F16), (2054, 16, 2, F32), (2560, 8, 1, BF16), (1600, 32, 2, F16), (1000, 64, 1, BF16), (160, 16, 1, F32), (1200, 16, 1, F16)])
+def test_ssm_seq_of_wide_layers(pkg, d, n, g, dtype):
+    """enough channels and sequences for every way of sharing the states among lanes"""
+    lengths = [40, 7, 0, 64, 1, 12]
+    starts = np.cumsum([0] + lengths).tolist()
+    x, dt, A, B, C, D, z, bias = _ssm_inputs(starts[-1], d, n, g, dtype)
+    for k in (6, 1):
+        st = starts[:k + 1]
+        pool = _rand(2 * k, d, n, seed=9)
+        p = pool.clone()
+        fro, to = [i if i % 3 else -1 for i in range(k)], [2 * k - 1 - i for i in range(k)]
+        got = pkg.ssm_seq(x, dt, A, B, C, D=D, z=z, dt_bias=bias, starts=st, state=p, from_slots=fro, to_slots=to)
+        y, ey, new, enew = _ssm_want(x, dt, A, B, C, D, z, bias, True, st, pool, fro, to)
+        _check(got[:st[-1]], y[:st[-1]], ey[:st[-1]], "out")
+        _check(p, new, enew, "state")
+
+
 @pytest.mark.parametrize("streams", [1, 3, 40, 600])
 @pytest.mark.parametrize("d,n,g,dtype", SSM_SHAPES)
 def test_ssm_step(pkg, streams, d, n, g, dtype):
