@@ -92,7 +92,8 @@ SIGNATURES = {
     "fr_b200_groupnorm": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "fr_b200_elementwise": (_i, [_i, _vp, _i, _vp, _i, _vp, _i, ctypes.c_float, _vp, _i, _sz, _vp]),
     "fr_b200_matmul": (_i, [_vp, _i, _i, _i, _vp, _i, _i, _vp, _i, _i, _vp]),
-    "fr_b200_linear": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i, _i, _vp, _i, _vp, _i64, _vp, _i64, _i, _i, _vp]),
+    "fr_b200_linear_workspace": (_sz, [_vp, _i64, _vp, _i64, _i64, _i, _i]),
+    "fr_b200_linear": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i, _i, _vp, _i, _vp, _i64, _vp, _i64, _i, _vp, _sz, _i, _vp]),
     "fr_b200_conv_seq": (_i, [_vp, _i64, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
     "fr_b200_conv_step": (_i, [_vp, _i64, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
     "fr_b200_ssm_seq_workspace": (_sz, [_i64, _i, _i, _i]),

@@ -86,24 +86,32 @@ __device__ __forceinline__ void mma_16816(float *d, const uint32_t *a, const uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// Rows that no tensor map takes (not a multiple of 16 bytes apart, or not starting at one): element by element into shared memory, 64 x 64 tiles.
+// More rows whose places no tensor map takes (not a multiple of 16 bytes apart, or not starting at one): element by element into shared memory,
+// 64 x 64 tiles.  Where there are few tiles, K is cut over the CTAs of a cluster, whose sums meet in shared memory in the pieces' order.
 constexpr int ANY_TILE = 64, ANY_K = 32, ANY_LD = ANY_K + 8;
+__device__ __forceinline__ float lds_cluster(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
 template <typename T>
-__global__ void __launch_bounds__(128) linear_any_kernel(const LinearArgs a) {
+__global__ void __launch_bounds__(128) linear_any_kernel(const LinearArgs a, int split) {
   __shared__ T s_x[ANY_TILE][ANY_LD], s_w[ANY_TILE][ANY_LD];
+  __shared__ float s_sum[ANY_TILE][ANY_TILE + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = split > 1 ? (int)cluster_rank() : 0;
   const long long m0 = (long long)blockIdx.y * ANY_TILE;
-  const int n0 = blockIdx.x * ANY_TILE;
+  const int n0 = blockIdx.x / split * ANY_TILE;
+  const int steps = (a.K + ANY_K - 1) / ANY_K, k_begin = (int)((long long)rank * steps / split) * ANY_K, k_end = (int)((long long)(rank + 1) * steps / split) * ANY_K;
   const T *x = reinterpret_cast<const T *>(a.x), *w = reinterpret_cast<const T *>(a.w);
   const int kc = tid % ANY_K, r0 = tid / ANY_K;   // column, first row; rows r0, r0 + 4, ...
   T px[16], pw[16];
-  auto fetch = [&](int k0) {
-    const bool kin = k0 + kc < a.K;
+  auto fetch = [&](int k0) {   // (past the end of rows the last one again, of columns too, but counted as zeros)
+    const int k = min(k0 + kc, a.K - 1);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int r = r0 + 4 * i;
-      px[i] = kin && m0 + r < a.M ? x[(m0 + r) * a.ldx + k0 + kc] : from_f<T>(0.f);
-      pw[i] = kin && n0 + r < a.N ? w[(long long)(n0 + r) * a.ldw + k0 + kc] : from_f<T>(0.f);
+      px[i] = x[min(m0 + r0 + 4 * i, (long long)a.M - 1) * a.ldx + k];
+      pw[i] = w[(long long)min(n0 + r0 + 4 * i, a.N - 1) * a.ldw + k];
     }
   };
   float acc[2][4][4];
@@ -114,14 +122,14 @@ __global__ void __launch_bounds__(128) linear_any_kernel(const LinearArgs a) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
   const int wm = (warp >> 1) * 32, wn = (warp & 1) * 32, gr = lane >> 2, gc = (lane & 3) * 2;
-  pdl_trigger();
   pdl_wait();
-  fetch(0);
-  for (int k0 = 0; k0 < a.K; k0 += ANY_K) {
+  fetch(k_begin);
+  for (int k0 = k_begin; k0 < k_end; k0 += ANY_K) {
+    const bool in = k0 + kc < a.K;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { s_x[r0 + 4 * i][kc] = px[i]; s_w[r0 + 4 * i][kc] = pw[i]; }
+    for (int i = 0; i < 16; ++i) { s_x[r0 + 4 * i][kc] = in ? px[i] : from_f<T>(0.f); s_w[r0 + 4 * i][kc] = in ? pw[i] : from_f<T>(0.f); }
     __syncthreads();
-    if (k0 + ANY_K < a.K) fetch(k0 + ANY_K);
+    fetch(k0 + ANY_K);
 #pragma unroll
     for (int kk = 0; kk < ANY_K; kk += 16) {
       uint32_t fa[2][4], fb[4][2];
@@ -146,16 +154,24 @@ __global__ void __launch_bounds__(128) linear_any_kernel(const LinearArgs a) {
     }
     __syncthreads();
   }
+  pdl_trigger();
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const long long m = m0 + wm + i * 16 + gr + (q >> 1) * 8;
-        const int n = n0 + wn + j * 8 + gc + (q & 1);
-        if (m < a.M && n < a.N) finish<T>(a, m, n, acc[i][j][q]);
-      }
+      for (int q = 0; q < 4; ++q) s_sum[wm + i * 16 + gr + (q >> 1) * 8][wn + j * 8 + gc + (q & 1)] = acc[i][j][q];
+  __syncthreads();
+  if (split > 1) cluster_sync();
+  for (int e = rank * 128 + tid; e < ANY_TILE * ANY_TILE; e += split * 128) {
+    const int r = e / ANY_TILE, c = e % ANY_TILE;
+    float v = 0.f;
+    if (split == 1) v = s_sum[r][c];
+    else
+      for (int q = 0; q < split; ++q) v += lds_cluster(mapa_u32(smem_u32(&s_sum[r][c]), q));
+    if (m0 + r < a.M && n0 + c < a.N) finish<T>(a, m0 + r, n0 + c, v);
+  }
+  if (split > 1) cluster_sync();
 }
 
 // ---- up to 32 rows of x ------------------------------------------------------------------------------------------
@@ -164,7 +180,7 @@ __global__ void __launch_bounds__(128) linear_any_kernel(const LinearArgs a) {
 // (which 16 of the 32 inputs an MMA adds up does not matter, as long as x and w agree), so no weight passes through shared memory
 // and all loads of a warp are in flight at once.  One row of 2048 x 8192: 7.5 us, 4.5 TB/s; through a TMA ring and tcgen05 10.4, whose set-up
 // and way through tensor memory 4 us of weights would have to hide.
-template <typename T, int NT, int NW, int CTAS>
+template <typename T, int NT, int NW, int CTAS, bool VEC>
 __global__ void __launch_bounds__(32 * NW, CTAS) linear_rows_kernel(const LinearArgs a) {
   constexpr int CH = 16, ROWS = 8 * NT, STEP = 32 * NW, U = 2;   // U steps in flight
   __shared__ float red[NW][ROWS][CH + 1];
@@ -191,27 +207,48 @@ __global__ void __launch_bounds__(32 * NW, CTAS) linear_rows_kernel(const Linear
       }
   };
   pdl_wait();
-  // whole pieces, then the last one: a load that may be narrower is waited for where its ways meet, one by one
+  // whole pieces, then the last one: a load that may be narrower is waited for where its ways meet, one by one.  Rows that are not whole 16 bytes apart
+  // (not VEC) come element by element, all of a step in flight: those past the end repeat the last one and count as zeros.
   int k0 = warp * 32;
-  for (; k0 + STEP * (U - 1) + 32 <= a.K; k0 += STEP * U) {
-    Frag w[U][2], x[U][NT];
+  if constexpr (VEC) {
+    for (; k0 + STEP * (U - 1) + 32 <= a.K; k0 += STEP * U) {
+      Frag w[U][2], x[U][NT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) w[u][i].p = *reinterpret_cast<const Pack<T, 8> *>(wp[i] + k0 + STEP * u);
+        for (int i = 0; i < 2; ++i) w[u][i].p = *reinterpret_cast<const Pack<T, 8> *>(wp[i] + k0 + STEP * u);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) x[u][j].p = *reinterpret_cast<const Pack<T, 8> *>(xp[j] + k0 + STEP * u);
+        for (int j = 0; j < NT; ++j) x[u][j].p = *reinterpret_cast<const Pack<T, 8> *>(xp[j] + k0 + STEP * u);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) multiply(w[u], x[u]);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) multiply(w[u], x[u]);
   }
   for (; k0 < a.K; k0 += STEP) {
     Frag w[2], x[NT];
     const int n = a.K - k0 - t * 8;
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w[i].p = load_some<T, 8>(wp[i] + k0, n, n >= 8);
+      for (int i = 0; i < 2; ++i) w[i].p = load_some<T, 8>(wp[i] + k0, n, n >= 8);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) x[j].p = load_some<T, 8>(xp[j] + k0, n, n >= 8);
+      for (int j = 0; j < NT; ++j) x[j].p = load_some<T, 8>(xp[j] + k0, n, n >= 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = k0 + min(e, n - 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i].p.v[e] = wp[i][at];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x[j].p.v[e] = xp[j][at];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e >= n) {
+          w[0].p.v[e] = w[1].p.v[e] = from_f<T>(0.f);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) x[j].p.v[e] = from_f<T>(0.f);
+        }
+    }
     multiply(w, x);
   }
   pdl_trigger();   // (not earlier: CTAs of the next kernel would crowd on the SMs that have few of this one's)
@@ -627,14 +664,18 @@ bool rows_map(CUtensorMap *map, const void *base, long long rows, int K, long lo
   const cuuint32_t box[2] = {(cuuint32_t)LK, (cuuint32_t)box_rows};
   return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, true, true);
 }
-template <typename T, int NT, int NW, int CTAS>
+template <typename T, int NT, int NW, int CTAS, bool VEC>
 cudaError_t rows_launch(const LinearArgs &a, cudaStream_t st) {
-  return op_launch(linear_rows_kernel<T, NT, NW, CTAS>, dim3((a.N + 15) / 16), 32 * NW, 0, st, 1, a);
+  return op_launch(linear_rows_kernel<T, NT, NW, CTAS, VEC>, dim3((a.N + 15) / 16), 32 * NW, 0, st, 1, a);
 }
 // 16 warps a CTA where there are few: up to two CTAs an SM.  One row of 5120 x 2560: 8.1 us (eight warps 10.8), of 2048 x 8192: 8.5 (7.6).
-template <typename T, int NT, int C8, int C16>
+template <typename T, int NT, int C8, int C16, bool VEC>
 cudaError_t rows_any(const LinearArgs &a, cudaStream_t st) {
-  return (a.N + 15) / 16 <= 2 * device_sm_count() ? rows_launch<T, NT, 16, C16>(a, st) : rows_launch<T, NT, 8, C8>(a, st);
+  return (a.N + 15) / 16 <= 2 * device_sm_count() ? rows_launch<T, NT, 16, C16, VEC>(a, st) : rows_launch<T, NT, 8, C8, VEC>(a, st);
+}
+template <typename T, bool VEC>
+cudaError_t rows_launch(const LinearArgs &a, cudaStream_t st) {
+  return a.M <= 8 ? rows_any<T, 1, 4, 2, VEC>(a, st) : a.M <= 16 ? rows_any<T, 2, 4, 2, VEC>(a, st) : rows_any<T, 4, 3, 1, VEC>(a, st);
 }
 template <typename T>
 cudaError_t tile_launch(const LinearArgs &a, int bn, int split, cudaStream_t st) {
@@ -678,6 +719,49 @@ cudaError_t pair_launch(const LinearArgs &a, int bn, cudaStream_t st) {
   return op_launch(kern, dim3(2 * pairs), LP_THREADS, LP_SMEM, st, 2, a, p, maps);
 }
 
+// rows of K 16-bit elements from wherever they start -> rows of whole 16 bytes, the rest of the last zeros: a word is cut out of the two that it lies in
+__global__ void __launch_bounds__(256) linear_align_kernel(const uint16_t *src, long long ld, long long rows, int K, uint4 *dst, int words) {
+  pdl_wait();
+  pdl_trigger();
+  const long long total = rows * words;
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
+    const long long r = e / words;
+    const int c = (int)(e - r * words) * 8, left = min(K - c, 8);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(src + r * ld + c);
+    const uint4 *w = reinterpret_cast<const uint4 *>(p & ~(uintptr_t)15);
+    const int off = (int)(p & 15), more = off + left * 2 > 16;
+    const uint4 a = w[0], b = w[more];
+    const uint32_t v[9] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, 0u};
+    uint32_t o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t lo = 0, hi = 0;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s == off / 4) { lo = v[q + s]; hi = v[q + s + 1]; }
+      const uint32_t x = __funnelshift_r(lo, hi, (off & 3) * 8);
+      o[q] = 2 * q + 1 < left ? x : 2 * q < left ? x & 0xffffu : 0u;
+    }
+    dst[e] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+bool whole_rows(const void *p, long long ld) { return ld % 8 == 0 && aligned(p, 16); }
+// bytes for copies of the operands that no tensor map takes, where a product is worth them: 100 x 5119 x 515 27 us element by element, 60 x 1001 x 777 7.5
+size_t align_bytes(const void *p, long long ld, long long rows, int K) { return whole_rows(p, ld) ? 0 : (size_t)rows * ((K + 7) / 8) * 16; }
+bool worth_aligning(long long M, int K, int N) { return M > 32 && (double)M * K * N >= 1.5e8; }
+cudaError_t align_launch(const void **p, long long *ld, long long rows, int K, uint8_t **work, cudaStream_t st) {
+  const size_t bytes = align_bytes(*p, *ld, rows, K);
+  if (!bytes) return cudaSuccess;
+  const int words = (K + 7) / 8;
+  const long long blocks = (rows * words + 255) / 256;
+  const cudaError_t e = op_launch(linear_align_kernel, dim3((unsigned)std::min<long long>(blocks, 16ll * device_sm_count())), 256, 0, st, 1,
+                                  reinterpret_cast<const uint16_t *>(*p), *ld, rows, K, reinterpret_cast<uint4 *>(*work), words);
+  *p = *work;
+  *ld = 8ll * words;
+  *work += bytes;
+  return e;
+}
+
 // Which kernel, which tile, how many pieces of K: the least of the times that these formulas give, in us, fitted to products of 27 to 4096 rows
 // with K x N = 2048 x 8192, 5120 x 2560, 2560 x 8960, 768 x 1536 and 160 x 5120.  Of 72 products of these and four other matrices the
 // choice was within 8 % of the fastest kernel, tile and cut for all but a few of 6 us that it made 7.
@@ -686,7 +770,7 @@ LinearChoice linear_choice(int M, int K, int N) {
   LinearChoice best{0, 0, 0, 0, 1e30f};
   // up to 16 rows the weights come straight to the registers; up to 32 those of small matrices (32 rows of 2048 x 2048 6.0 us against 8.3,
   // of 5120 x 2560 14.7 against 11.6)
-  if (M <= 16 || (M <= 32 && (long long)K * N <= 5 << 20)) { best.rows = M <= 8 ? 8 : M <= 16 ? 16 : 32; return best; }
+  if (M <= 16 || (M <= 32 && (long long)K * N <= 5 << 20)) { best.rows = 1; return best; }
   const int nk = (K + LK - 1) / LK, sms = device_sm_count(), ct = (N + 127) / 128;
   const float stream = 2.f * K * N / 6.2e6f;   // the weights at the card's bandwidth
   auto take = [&](float us, int pair, int bn, int split) {
@@ -715,30 +799,42 @@ LinearChoice linear_choice(int M, int K, int N) {
 
 template <typename T>
 cudaError_t any_launch(const LinearArgs &a, cudaStream_t st) {
-  return op_launch(linear_any_kernel<T>, dim3((a.N + ANY_TILE - 1) / ANY_TILE, (a.M + ANY_TILE - 1) / ANY_TILE), 128, 0, st, 1, a);
+  const int nt = (a.N + ANY_TILE - 1) / ANY_TILE, mt = (a.M + ANY_TILE - 1) / ANY_TILE, steps = (a.K + ANY_K - 1) / ANY_K;
+  int split = 1;   // two CTAs an SM, four steps each at least
+  while (split < 8 && (long long)nt * mt * split * 2 <= 2 * device_sm_count() && steps >= split * 8) split *= 2;
+  return op_launch(linear_any_kernel<T>, dim3(nt * split, mt), 128, 0, st, split, a, split);
 }
 template <typename T>
-cudaError_t linear_launch(const LinearArgs &a, cudaStream_t st) {
-  const bool whole = a.ldx % 8 == 0 && a.ldw % 8 == 0 && aligned(a.x, 16) && aligned(a.w, 16);
-  if (!whole) return any_launch<T>(a, st);
+cudaError_t linear_launch(LinearArgs a, uint8_t *work, cudaStream_t st) {
+  if (work) {
+    cudaError_t e = align_launch(&a.x, &a.ldx, a.M, a.K, &work, st);
+    if (e == cudaSuccess) e = align_launch(&a.w, &a.ldw, a.N, a.K, &work, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (!whole_rows(a.x, a.ldx) || !whole_rows(a.w, a.ldw)) return a.M <= 32 ? rows_launch<T, false>(a, st) : any_launch<T>(a, st);
   const LinearChoice c = linear_choice(a.M, a.K, a.N);
-  if (c.rows == 8) return rows_any<T, 1, 4, 2>(a, st);
-  if (c.rows == 16) return rows_any<T, 2, 4, 2>(a, st);
-  if (c.rows == 32) return rows_any<T, 4, 3, 1>(a, st);
+  if (c.rows) return rows_launch<T, true>(a, st);
   return c.pair ? pair_launch<T>(a, c.bn, st) : tile_launch<T>(a, c.bn, c.split, st);
 }
 
 }  // namespace
 
+constexpr int64_t LINEAR_ROWS = 65535ll * ANY_TILE;   // what a grid takes
+
 extern "C" {
 
+size_t fr_b200_linear_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t rows, int K, int N) {
+  if (rows < 1 || K < 1 || N < 1 || !worth_aligning(rows, K, N)) return 0;
+  return align_bytes(x, ldx, rows, K) + align_bytes(w, ldw, N, K);
+}
+
 int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, int64_t rows, int K, int N, const float *bias, int act,
-                   const void *residual, int64_t ldr, void *out, int64_t ldo, int out_dtype, int device, void *stream) {
+                   const void *residual, int64_t ldr, void *out, int64_t ldo, int out_dtype, void *work, size_t work_bytes, int device, void *stream) {
   OP_TRY
   OP_REQUIRE(dtype == FR_B200_T_F16 || dtype == FR_B200_T_BF16, "x and w are f16 or bf16");
   OP_REQUIRE(out_dtype == dtype || out_dtype == FR_B200_T_F32, "out has the type of x, or f32");
   OP_REQUIRE(act >= FR_B200_ACT_NONE && act <= FR_B200_ACT_SOFTPLUS, "unknown activation");
-  OP_REQUIRE(rows >= 0 && rows <= (1 << 22) && K >= 1 && N >= 1, "bad shape");
+  OP_REQUIRE(rows >= 0 && rows <= LINEAR_ROWS && K >= 1 && K <= (1 << 24) && N >= 1 && N <= (1 << 24), "bad shape");
   OP_REQUIRE(ldx >= K && ldw >= K && ldo >= N && (!residual || ldr >= N), "rows are closer than they are long");
   if (rows == 0) return FR_B200_OK;
   OP_REQUIRE(x && w && out, "null tensor");
@@ -749,6 +845,8 @@ int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int d
   OP_REQUIRE(!overlap(ro, Rows{bias, 4 * (int64_t)N, 4 * (int64_t)N, bias ? 1 : 0}), "out overlaps the bias");
   OP_REQUIRE((residual == out && ldr == ldo) || !overlap(ro, Rows{residual, ldr * os, (int64_t)N * os, residual ? rows : 0}),
              "the residual overlaps out without being it");
+  const size_t need = fr_b200_linear_workspace(x, ldx, w, ldw, rows, K, N);
+  OP_REQUIRE(!work || (aligned(work, 16) && work_bytes >= need), "the work area is smaller than fr_b200_linear_workspace() or not at 16 bytes");
   DeviceScope dev;
   OP_CU(dev.enter(device));
   LinearArgs a{x, w, residual, bias, out, ldx, ldw, ldr, ldo, (int)rows, N, K, act, out_dtype == FR_B200_T_F32};
@@ -757,8 +855,8 @@ int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int d
     linear_status = 0;
     return op_fail(FR_B200_E_TIMEOUT, "a wait of an earlier linear call gave up; its result is not there");
   }
-  if (dtype == FR_B200_T_F16) OP_CU(linear_launch<__half>(a, st));
-  else OP_CU(linear_launch<__nv_bfloat16>(a, st));
+  if (dtype == FR_B200_T_F16) OP_CU(linear_launch<__half>(a, need ? reinterpret_cast<uint8_t *>(work) : nullptr, st));
+  else OP_CU(linear_launch<__nv_bfloat16>(a, need ? reinterpret_cast<uint8_t *>(work) : nullptr, st));
   return FR_B200_OK;
   OP_CATCH
 }

@@ -237,7 +237,7 @@ cudaError_t conv_any(int dt, int taps, const ConvArgs &a, const TAB &t, int vec,
 int conv_check(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const float *w, int taps, const float *bias, int act, void *state,
                int64_t state_stride, int n_slots, void *out, int64_t ldo, ConvArgs *a, int *vec) {
   OP_REQUIRE(dt_known(dtype), "dtype must be f16, bf16 or f32");
-  OP_REQUIRE(rows >= 0 && D >= 1 && ldx >= D && ldo >= D, "bad shape");
+  OP_REQUIRE(rows >= 0 && D >= 1 && D <= (1 << 24) && ldx >= D && ldo >= D, "bad shape");
   OP_REQUIRE(rows < (1ll << 31), "too many rows");
   OP_REQUIRE(taps >= 2 && taps <= 4, "2 to 4 taps");
   OP_REQUIRE(act == FR_B200_ACT_NONE || act == FR_B200_ACT_SILU, "the convolution's activation is none or silu");
@@ -257,15 +257,17 @@ int conv_check(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const
 }
 
 // ---- the selective state space scan (sequences: ssm.cuh) ----------------------------------------------------------
-// One token of each stream: L lanes a channel, four states a lane (and every 4 L-th four), CPT channels a thread, whose states are all asked
-// for at once.  Bound by reading and writing the states.
-template <typename T, int L, int CPT, bool VEC>
-__global__ void __launch_bounds__(128) ssm_step_kernel(const SsmArgs a, const __grid_constant__ SlotTable tab) {
-  constexpr int CH = 128 / L;
+// One token of each stream.  L lanes share CPT neighbouring channels, four states of each a lane (and every 4 L-th four): their states are all asked for
+// at once.  Each of the first CPT lanes brings x, dt and z of one channel, makes its time step for the others, and ends with its sum over
+// the states.  Bound by reading and writing the states: 256 streams of 4096 channels with 16 states 134 MB; with x, dt, z and the time
+// step made by every lane it was bound by 708 instructions a warp.
+template <typename T, int L, bool VEC>
+__global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const __grid_constant__ SlotTable tab) {
+  constexpr int CPT = L < 4 ? L : 4, CH = 128 / L * CPT;
   const int lane = threadIdx.x % L, s = blockIdx.y;
   // the channels of a CTA are of one group
-  const int per_group = a.d / a.groups, ctas = (per_group + CH * CPT - 1) / (CH * CPT), group = blockIdx.x / ctas;
-  const int ch_end = (group + 1) * per_group, ch0 = group * per_group + (blockIdx.x - group * ctas) * (CH * CPT) + threadIdx.x / L;
+  const int per_group = a.d / a.groups, ctas = (per_group + CH - 1) / CH, group = blockIdx.x / ctas;
+  const int ch_end = (group + 1) * per_group, ch0 = group * per_group + (blockIdx.x - group * ctas) * CH + threadIdx.x / L * CPT;
   const long long row = tab.base + s;
   const int from_slot = tab.from[s], to_slot = tab.to[s];
   pdl_wait();
@@ -274,63 +276,80 @@ __global__ void __launch_bounds__(128) ssm_step_kernel(const SsmArgs a, const __
   float *to = a.state + (long long)max(to_slot, 0) * a.state_stride;
   const T *bp = reinterpret_cast<const T *>(a.B) + row * a.ldb + (long long)group * a.n;
   const T *cp = reinterpret_cast<const T *>(a.C) + row * a.ldc + (long long)group * a.n;
-  const T *zp = a.z ? reinterpret_cast<const T *>(a.z) + row * a.ldz : reinterpret_cast<const T *>(a.x) + row * a.ldx;
-  int c[CPT];
+  int at[CPT];   // a channel's states (channels past the end: the last one's again, not kept)
 #pragma unroll
-  for (int k = 0; k < CPT; ++k) c[k] = min(ch0 + k * CH, ch_end - 1);   // (channels past the end: computed, not kept)
-  float y[CPT], x[CPT], delta[CPT], z[CPT], skip[CPT];
-  for (int n = min(lane * 4, a.n - 1), first = 1; n < a.n && lane * 4 < a.n; n += 4 * L, first = 0) {
-    const int left = min(a.n - n, 4);
+  for (int k = 0; k < CPT; ++k) at[k] = min(ch0 + k, ch_end - 1) * a.n;
+  const int mine = min(ch0 + lane % CPT, ch_end - 1);
+  const float x = to_f(reinterpret_cast<const T *>(a.x)[row * a.ldx + mine]), dt = to_f(reinterpret_cast<const T *>(a.dt)[row * a.lddt + mine]);
+  const float z = a.z ? to_f(reinterpret_cast<const T *>(a.z)[row * a.ldz + mine]) : 0.f;
+  const float bias = a.dt_bias ? a.dt_bias[mine] : 0.f, skip = a.D ? a.D[mine] : 0.f;
+  float delta = 0.f, u = 0.f, y[CPT];
+#pragma unroll
+  for (int k = 0; k < CPT; ++k) y[k] = 0.f;
+  for (int n0 = 0; n0 < a.n; n0 += 4 * L) {
+    const int n = n0 + lane * 4, there = a.n - n, left = VEC ? 4 : min(max(there, 1), 4), nc = VEC ? min(n, a.n - 4) : min(n, a.n - 1);
     Pack<float, 4> h[CPT], A4[CPT];
 #pragma unroll
-    for (int k = 0; k < CPT; ++k) {
+    for (int k = 0; k < CPT; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) h[k].v[i] = 0.f;
-      if (from_slot >= 0) h[k] = load_pack<float, 4, VEC>(from + (size_t)c[k] * a.n + n, left);
+    if (from_slot >= 0)
+#pragma unroll
+      for (int k = 0; k < CPT; ++k) h[k] = load_pack<float, 4, VEC>(from + at[k] + nc, left);
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) A4[k] = load_pack<float, 4, VEC>(a.A + at[k] + nc, left);
+    const Pack<T, 4> B = load_pack<T, 4, false>(bp + nc, left), C = load_pack<T, 4, false>(cp + nc, left);
+    if (n0 == 0) {
+      const float v = dt + bias;
+      delta = a.softplus ? softplus(v) : v;
+      u = delta * x;
     }
+    unsigned long long b[2], c[2];
 #pragma unroll
-    for (int k = 0; k < CPT; ++k) A4[k] = load_pack<float, 4, VEC>(a.A + (size_t)c[k] * a.n + n, left);
-    const Pack<T, 4> B = load_pack<T, 4, false>(bp + n, left), C = load_pack<T, 4, false>(cp + n, left);
-    if (first)
-#pragma unroll
-      for (int k = 0; k < CPT; ++k) {
-        x[k] = to_f(reinterpret_cast<const T *>(a.x)[row * a.ldx + c[k]]);
-        float d = to_f(reinterpret_cast<const T *>(a.dt)[row * a.lddt + c[k]]) + (a.dt_bias ? a.dt_bias[c[k]] : 0.f);
-        z[k] = to_f(zp[c[k]]);
-        skip[k] = a.D ? a.D[c[k]] : 0.f;
-        delta[k] = a.softplus ? softplus(d) : d;
-        y[k] = 0.f;
-      }
+    for (int q = 0; q < 2; ++q) {
+      b[q] = pack_f2(to_f(B.v[2 * q]), to_f(B.v[2 * q + 1]));
+      c[q] = pack_f2(2 * q < there ? to_f(C.v[2 * q]) : 0.f, 2 * q + 1 < there ? to_f(C.v[2 * q + 1]) : 0.f);
+    }
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
-      const float d = delta[k] * LOG2E, u = delta[k] * x[k];
+      const float dk = L == 1 ? delta : __shfl_sync(0xffffffffu, delta, k, L), uk = L == 1 ? u : __shfl_sync(0xffffffffu, u, k, L), d2 = dk * LOG2E;
+      unsigned long long ys = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[k].v[i] = fmaf(ex2(d * A4[k].v[i]), h[k].v[i], u * to_f(B.v[i]));
-        if (i < left) y[k] = fmaf(h[k].v[i], to_f(C.v[i]), y[k]);
+      for (int q = 0; q < 2; ++q) {
+        float e0, e1;
+        unpack_f2(mul_f2(pack_f2(d2, d2), pack_f2(A4[k].v[2 * q], A4[k].v[2 * q + 1])), e0, e1);
+        const unsigned long long hs = fma_f2(pack_f2(ex2(e0), ex2(e1)), pack_f2(h[k].v[2 * q], h[k].v[2 * q + 1]), mul_f2(pack_f2(uk, uk), b[q]));
+        ys = q ? fma_f2(hs, c[q], ys) : mul_f2(hs, c[q]);
+        unpack_f2(hs, h[k].v[2 * q], h[k].v[2 * q + 1]);
       }
-      if (to_slot >= 0 && ch0 + k * CH < ch_end) store_pack<float, 4, VEC>(to + (size_t)c[k] * a.n + n, h[k], left);
+      float y0, y1;
+      unpack_f2(ys, y0, y1);
+      y[k] += there > 0 ? y0 + y1 : 0.f;
+      if (to_slot >= 0 && ch0 + k < ch_end && there > 0) store_pack<float, 4, VEC>(to + at[k] + nc, h[k], left);
     }
   }
+  // over the lanes: those that hold the same four channels, then each keeps one channel's
 #pragma unroll
-  for (int k = 0; k < CPT; ++k) {
-    if (lane * 4 >= a.n) y[k] = x[k] = z[k] = skip[k] = 0.f;   // a lane without states
+  for (int o = L / 2; o >= CPT; o >>= 1)
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
-    y[k] = fmaf(skip[k], x[k], y[k]);
-    if (a.z) y[k] *= silu(z[k]);
-    if (lane == 0 && ch0 + k * CH < ch_end) reinterpret_cast<T *>(a.out)[row * a.ldo + c[k]] = from_f<T>(y[k]);
+    for (int k = 0; k < CPT; ++k) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+#pragma unroll
+  for (int o = CPT / 2; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int k = 0; k < o; ++k) {
+      const float send = up ? y[k] : y[k + o], keep = up ? y[k + o] : y[k];
+      y[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
   }
+  float out = fmaf(skip, x, y[0]);
+  if (a.z) out *= silu(z);
+  if (lane < CPT && ch0 + lane < ch_end) reinterpret_cast<T *>(a.out)[row * a.ldo + ch0 + lane] = from_f<T>(out);
 }
-
-// four channels a thread where that leaves every SM a few CTAs, else one
 template <typename T, int L, bool VEC>
 cudaError_t ssm_step_launch(const SsmArgs &a, const SlotTable &t, cudaStream_t st) {
-  constexpr int CH = 128 / L;
-  const int per_group = a.d / a.groups;
-  auto grid = [&](int ch) { return dim3((per_group + ch - 1) / ch * a.groups, t.n); };
-  if ((long long)a.d * t.n >= 148ll * 4 * 4 * CH) return op_launch(ssm_step_kernel<T, L, 4, VEC>, grid(4 * CH), 128, 0, st, 1, a, t);
-  return op_launch(ssm_step_kernel<T, L, 1, VEC>, grid(CH), 128, 0, st, 1, a, t);
+  constexpr int CH = 128 / L * (L < 4 ? L : 4);
+  return op_launch(ssm_step_kernel<T, L, VEC>, dim3((a.d / a.groups + CH - 1) / CH * a.groups, t.n), 128, 0, st, 1, a, t);
 }
 template <typename T, bool VEC>
 cudaError_t ssm_step_any(const SsmArgs &a, const SlotTable &t, cudaStream_t st) {
@@ -345,7 +364,7 @@ constexpr int SSM_STATES = 128;   // most states of a channel
 
 int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots) {
   OP_REQUIRE(dt_known(dtype), "dtype must be f16, bf16 or f32");
-  OP_REQUIRE(rows >= 0 && rows < (1ll << 31) && a.d >= 1, "bad shape");
+  OP_REQUIRE(rows >= 0 && rows < (1ll << 31) && a.d >= 1 && a.d <= (1 << 23), "bad shape");
   OP_REQUIRE(a.n >= 1 && a.n <= SSM_STATES, "1 to 128 states a channel");
   OP_REQUIRE(a.groups >= 1 && a.d % a.groups == 0, "the channels are not a multiple of the groups");
   const int64_t bn = (int64_t)a.groups * a.n;

@@ -15,6 +15,7 @@
 namespace {
 
 decltype(&fr_b200_linear) p_linear;
+decltype(&fr_b200_linear_workspace) p_linear_workspace;
 decltype(&fr_b200_conv_seq) p_conv_seq;
 decltype(&fr_b200_conv_step) p_conv_step;
 decltype(&fr_b200_ssm_seq) p_ssm_seq;
@@ -184,6 +185,8 @@ struct Place {
   void *stream;
   explicit Place(const at::Tensor &x) : device(x.get_device()), stream(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)x.get_device()).stream()) {}
 };
+// Scratch of a call.  It goes back to the allocator behind the call: what gets it next on this stream comes after.
+at::Tensor work_area(size_t bytes, const at::Tensor &x) { return bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : at::Tensor(); }
 // a tensor, or the negative status
 PyObject *answer(int rc, const at::Tensor &t) { return rc < 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(t); }
 
@@ -224,8 +227,11 @@ PyObject *py_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Rows rr = rows_of(res, "the residual", channels, nullptr);
     const float *bias = param(a[2], "bias", channels, -1, x);
     const Place at(x);
-    return answer(p_linear(xr.p, xr.ld, wr.p, wr.ld, dt, rows, fit(k, "x"), fit(channels, "w"), bias, (int)PyLong_AsLong(a[3]), rr.p, rr.ld, orow.p, orow.ld,
-                           out_dt, at.device, at.stream), out);
+    const int ki = fit(k, "x"), ni = fit(channels, "w");
+    const size_t need = p_linear_workspace(xr.p, xr.ld, wr.p, wr.ld, rows, ki, ni);
+    const at::Tensor work = work_area(need, x);
+    return answer(p_linear(xr.p, xr.ld, wr.p, wr.ld, dt, rows, ki, ni, bias, (int)PyLong_AsLong(a[3]), rr.p, rr.ld, orow.p, orow.ld, out_dt,
+                           need ? work.data_ptr() : nullptr, need, at.device, at.stream), out);
   });
 }
 
@@ -298,8 +304,7 @@ PyObject *py_ssm(PyObject *, PyObject *const *a, Py_ssize_t n) {
       return answer(p_ssm_step(xr.p, xr.ld, tr.p, tr.ld, Ap, br.p, br.ld, cr.p, cr.ld, skip, zr.p, zr.ld, bias, softplus, dt, fit(rows, "x"), di, ni, gi,
                                static_cast<float *>(pool.p), pool.stride, pool.slots, from.p, to.p, orow.p, orow.ld, at.device, at.stream), out);
     const size_t need = p_ssm_workspace(rows, fit(streams, "starts"), di, ni);
-    at::Tensor work;   // (handed back to the allocator behind the call: what gets it next on this stream comes after)
-    if (need) work = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
+    const at::Tensor work = work_area(need, x);
     return answer(p_ssm_seq(xr.p, xr.ld, tr.p, tr.ld, Ap, br.p, br.ld, cr.p, cr.ld, skip, zr.p, zr.ld, bias, softplus, dt, rows, di, ni, gi, starts.p,
                             (int)streams, static_cast<float *>(pool.p), pool.stride, pool.slots, from.p, to.p, orow.p, orow.ld,
                             need ? work.data_ptr() : nullptr, need, at.device, at.stream), out);
@@ -335,6 +340,7 @@ PyObject *py_bind(PyObject *, PyObject *path) {
   bool ok = true;
   auto get = [&](auto &f, const char *name) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(dlsym(h, name)); ok = ok && f; };
   get(p_linear, "fr_b200_linear");
+  get(p_linear_workspace, "fr_b200_linear_workspace");
   get(p_conv_seq, "fr_b200_conv_seq");
   get(p_conv_step, "fr_b200_conv_step");
   get(p_ssm_seq, "fr_b200_ssm_seq");

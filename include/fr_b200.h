@@ -274,7 +274,8 @@ const char *fr_b200_op_last_error(void);
  * the streams' states (the reference has none of them; they stand beside its recurrences above).  Common to all:
  *   - tensors are [rows, width] pieces whose rows lie `ld` elements apart; dtype FR_B200_T_F16, _BF16 or _F32; parameters
  *     (bias, weights of the convolution, A, D, dt_bias) are fp32.  Sums, states and statistics are fp32, each output is
- *     rounded once.  No alignment beyond the element's is asked; rows and pointers of whole 16 bytes are faster;
+ *     rounded once.  No alignment beyond the element's is asked; rows and pointers of whole 16 bytes are faster.  Up to
+ *     2^24 channels (2^23 of a scan);
  *   - asynchronous on `stream`, on `device` whatever device is current (the caller's stays current); nothing is allocated,
  *     nothing is synchronised, no result depends on the order of atomics: calls may be captured, and captured calls hold
  *     the host arrays (sequences, slots) by value;
@@ -289,9 +290,12 @@ const char *fr_b200_op_last_error(void);
 
 /* out[rows, N] = residual + act(x[rows, K] . w[N, K]^T + bias[N]); bias and residual may be NULL.  x, w: f16 or bf16 (the
  * same); out and residual: the type of x, or f32.  residual may be out itself.  Operands multiply on the tensor cores with
- * fp32 sums whose order depends on the shape alone; up to 4,194,304 rows. */
+ * fp32 sums whose order depends on shapes and alignment alone; up to 4,194,240 rows.  work: fr_b200_linear_workspace() bytes of
+ * device memory (at 16 bytes) that the call has to itself, for larger products whose rows are not whole 16 bytes apart (0 for
+ * others); NULL: such a product is taken element by element, several times slower. */
+size_t fr_b200_linear_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t rows, int K, int N);
 int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, int64_t rows, int K, int N, const float *bias, int act,
-                   const void *residual, int64_t ldr, void *out, int64_t ldo, int out_dtype, int device, void *stream);
+                   const void *residual, int64_t ldr, void *out, int64_t ldo, int out_dtype, void *work, size_t work_bytes, int device, void *stream);
 
 /* y[t, d] = act(bias[d] + sum_j w[d, j] x[t - (taps - 1) + j, d]), act none or silu, taps 2 to 4; w [D, taps], bias [D] or NULL.
  * A state is the last taps - 1 rows, [taps - 1, D] in the type of x, oldest first: they come before a sequence's first row. */

@@ -98,8 +98,8 @@ def test_linear_activations(pkg, act, rows, k, n):
         _check(pkg.linear(x, w, b, activation=act, out_dtype=out_dtype), want, err, act)
 
 
-@pytest.mark.parametrize("rows,k,n", [(1, 256, 64), (40, 256, 64), (300, 192, 136), (300, 191, 135)])
-@pytest.mark.parametrize("shift", [0, 1, 8])
+@pytest.mark.parametrize("rows,k,n", [(1, 256, 64), (12, 255, 65), (40, 256, 64), (300, 192, 136), (300, 191, 135), (520, 703, 650), (520, 704, 648)])
+@pytest.mark.parametrize("shift", [0, 1, 3, 8])
 def test_linear_pieces_of_wider_rows(pkg, rows, k, n, shift):
     """x, w, residual and out as columns of wider tensors, at 16-byte boundaries and off them; what lies beside out stays."""
     X, W, R = _rand(rows, k + 24, dtype=F16), _rand(n, k + 40, dtype=F16, scale=0.1, seed=1), _rand(rows, n + 16, dtype=F16, seed=2)
@@ -172,6 +172,23 @@ def test_linear_rows_do_not_depend_on_their_neighbours(pkg):
     x2 = x.clone()
     x2[150:] = float("nan")
     assert torch.equal(pkg.linear(x2, w)[:150], y[:150])
+
+
+def test_linear_without_a_work_area(pkg):
+    """a larger product off the 16-byte boundaries through the C entry, with scratch and without"""
+    rows, k, n = 130, 1501, 900
+    x, w = _rand(rows, k, dtype=BF16), _rand(n, k, dtype=BF16, scale=0.03, seed=1)
+    want, err = _linear_want(x, w, None, "none", None)
+    L = pkg.lib()
+    need = L.fr_b200_linear_workspace(x.data_ptr(), k, w.data_ptr(), k, rows, k, n)
+    assert need == (rows + n) * 188 * 16
+    assert L.fr_b200_linear_workspace(x.data_ptr(), 1504, w.data_ptr(), 1504, rows, k, n) == 0 and L.fr_b200_linear_workspace(x.data_ptr(), k, w.data_ptr(), k, 32, k, n) == 0
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for p, b in ((None, 0), (work.data_ptr(), need)):
+        out = torch.empty((rows, n), dtype=BF16, device="cuda")
+        rc = L.fr_b200_linear(x.data_ptr(), k, w.data_ptr(), k, 2, rows, k, n, None, 0, None, 0, out.data_ptr(), n, 2, p, b, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        _check(out, want, err)
 
 
 def test_linear_without_rows(pkg):

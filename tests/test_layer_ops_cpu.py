@@ -21,18 +21,19 @@ def _refused(pkg, name, args, word):
 
 
 def _linear(**kw):
-    a = dict(x=X, ldx=64, w=W, ldw=64, dtype=F16, rows=4, K=64, N=32, bias=None, act=0, residual=None, ldr=0, out=O, ldo=32, out_dtype=F16, device=0,
-             stream=None)
+    a = dict(x=X, ldx=64, w=W, ldw=64, dtype=F16, rows=4, K=64, N=32, bias=None, act=0, residual=None, ldr=0, out=O, ldo=32, out_dtype=F16, work=None, work_bytes=0,
+             device=0, stream=None)
     a.update(kw)
     return tuple(a.values())
 
 
 @pytest.mark.parametrize("kw,word", [
     (dict(dtype=F32), "f16 or bf16"), (dict(dtype=9), "f16 or bf16"), (dict(out_dtype=BF16), "out has the type"), (dict(act=6), "activation"),
-    (dict(act=-1), "activation"), (dict(K=0), "shape"), (dict(N=0), "shape"), (dict(rows=-1), "shape"), (dict(rows=(1 << 22) + 1), "shape"),
+    (dict(act=-1), "activation"), (dict(K=0), "shape"), (dict(N=0), "shape"), (dict(rows=-1), "shape"), (dict(rows=65535 * 64 + 1), "shape"), (dict(N=(1 << 24) + 1, ldo=1 << 25), "shape"), (dict(K=(1 << 24) + 1, ldx=1 << 25, ldw=1 << 25), "shape"),
     (dict(ldx=63), "closer"), (dict(ldw=0), "closer"), (dict(ldo=31), "closer"), (dict(residual=R, ldr=31), "closer"), (dict(x=None), "null"),
     (dict(w=None), "null"), (dict(out=None), "null"), (dict(x=X + 1), "misaligned"), (dict(bias=R + 2), "misaligned"),
     (dict(out_dtype=F32, out=O + 2), "misaligned"), (dict(out=X), "overlaps x"), (dict(out=W + 64), "overlaps x"), (dict(out=X + 2 * 64 * 3), "overlaps x"),
+    (dict(rows=4000, K=1001, ldx=1001, ldw=1001, N=100, ldo=100, out=O, work=S, work_bytes=4100 * 126 * 16 - 1), "work area"), (dict(work=S + 8, work_bytes=99), "work area"),
     (dict(bias=O), "bias"), (dict(residual=O + 2, ldr=32), "residual"), (dict(residual=O, ldr=40), "residual"),
 ])
 def test_linear_refuses(pkg, kw, word):
@@ -52,7 +53,7 @@ SLOTS = [(dict(fro=_i32(4), to=_i32(0)), "read is out of range"), (dict(fro=_i32
 
 
 @pytest.mark.parametrize("kw,word", SLOTS + [
-    (dict(dtype=3), "dtype"), (dict(taps=1), "taps"), (dict(taps=5), "taps"), (dict(act=1), "none or silu"), (dict(D=0), "shape"), (dict(rows=-1), "shape"),
+    (dict(dtype=3), "dtype"), (dict(taps=1), "taps"), (dict(taps=5), "taps"), (dict(act=1), "none or silu"), (dict(D=0), "shape"), (dict(D=(1 << 24) + 1), "shape"), (dict(rows=-1), "shape"),
     (dict(rows=1 << 31), "rows"), (dict(ldx=63), "shape"), (dict(ldo=63), "shape"), (dict(w=None), "null"), (dict(x=None), "null"), (dict(out=None), "null"),
     (dict(out=O + 1), "misaligned"), (dict(out=X + 128), "out overlaps"), (dict(out=S), "pool"), (dict(x=S + 128), "pool"),
     (dict(n_seq=2), "first rows"), (dict(n_seq=-1), "negative"), (dict(starts=_i32(-1, 5)), "outside"), (dict(starts=_i32(0, 21)), "outside"),
@@ -87,7 +88,7 @@ def _ssm(seq=True, **kw):
 
 
 SSM = [(dict(fro=_i32(4)), "read is out of range"), (dict(to=_i32(4)), "write is out of range"), (dict(state=None, n_slots=0, to=_i32(0)), "without a pool"),
-       (dict(state_stride=1023), "smaller"), (dict(state=S + 2), "misaligned"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "shape"), (dict(d=0), "shape"),
+       (dict(state_stride=1023), "smaller"), (dict(state=S + 2), "misaligned"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "shape"), (dict(d=0), "shape"), (dict(d=(1 << 23) + 1), "shape"),
        (dict(n=0), "states"), (dict(n=129), "states"), (dict(groups=0), "groups"), (dict(groups=3), "groups"), (dict(ldx=63), "closer"),
        (dict(lddt=1), "closer"), (dict(ldb=15), "closer"), (dict(ldc=31, groups=2), "closer"), (dict(z=R, ldz=63), "closer"), (dict(A=None), "null"),
        (dict(dt=None), "null"), (dict(B=None), "null"), (dict(out=None), "null"), (dict(out=O + 1), "misaligned"), (dict(A=W + 2), "misaligned"),
