@@ -92,11 +92,16 @@ template <int W, int V, bool VEC>
 struct ConvTaps {
   float w[V * W], b[V];
   __device__ __forceinline__ void load(const ConvArgs &a, int c, int n) {
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < V * W; i += 4) {
-      const Pack<float, 4> v = load_pack<float, 4, VEC>(a.w + (size_t)c * W + i, max(n * W - i, 1));
+      for (int i = 0; i < V * W; i += 4) {
+        const Pack<float, 4> v = load_pack<float, 4, true>(a.w + (size_t)c * W + i, 4);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) w[i + q] = v.v[q];
+        for (int q = 0; q < 4; ++q) w[i + q] = v.v[q];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V * W; ++i) w[i] = a.w[(size_t)c * W + min(i, n * W - 1)];   // (channels past the end: the last weight, not kept)
     }
     const Pack<float, 4> v = load_pack<float, 4, VEC>(a.bias ? a.bias + c : a.w, n);   // (no bias: something that is there, and not taken)
 #pragma unroll
@@ -319,8 +324,10 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
         float e0, e1;
         unpack_f2(mul_f2(pack_f2(d2, d2), pack_f2(A4[k].v[2 * q], A4[k].v[2 * q + 1])), e0, e1);
         const unsigned long long hs = fma_f2(pack_f2(ex2(e0), ex2(e1)), pack_f2(h[k].v[2 * q], h[k].v[2 * q + 1]), mul_f2(pack_f2(uk, uk), b[q]));
-        ys = q ? fma_f2(hs, c[q], ys) : mul_f2(hs, c[q]);
         unpack_f2(hs, h[k].v[2 * q], h[k].v[2 * q + 1]);
+        unsigned long long hc = hs;   // (states past the end: the last one's again, which may be infinite, and no 0 x inf is added)
+        if constexpr (!VEC) hc = pack_f2(2 * q < there ? h[k].v[2 * q] : 0.f, 2 * q + 1 < there ? h[k].v[2 * q + 1] : 0.f);
+        ys = q ? fma_f2(hc, c[q], ys) : mul_f2(hc, c[q]);
       }
       float y0, y1;
       unpack_f2(ys, y0, y1);
@@ -342,7 +349,7 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
       y[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
   }
-  float out = fmaf(skip, x, y[0]);
+  float out = a.D ? fmaf(skip, x, y[0]) : y[0];
   if (a.z) out *= silu(z);
   if (lane < CPT && ch0 + lane < ch_end) reinterpret_cast<T *>(a.out)[row * a.ldo + ch0 + lane] = from_f<T>(out);
 }

@@ -48,7 +48,6 @@ struct SsmTile {
 };
 // named barriers, two of each: rows put down; states done with them; rows finished (their buffers are free)
 enum { SSM_BAR_FULL = 1, SSM_BAR_DONE = 3, SSM_BAR_FREE = 5, SSM_BAR_IN = 7 };
-__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 template <int ID, int N> __device__ __forceinline__ void pair_sync(int which) { if (which) asm volatile("bar.sync %0, %1;" ::"n"(ID + 1), "n"(N) : "memory"); else asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
 template <int ID, int N> __device__ __forceinline__ void pair_arrive(int which) { if (which) asm volatile("bar.arrive %0, %1;" ::"n"(ID + 1), "n"(N) : "memory"); else asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
 __device__ __forceinline__ void copy_async16(void *dst, const void *src) {
@@ -105,7 +104,8 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
       A2[i] = pack_f2(av, av);
       h[i] = there && slot ? slot[(size_t)ch * a.n + n0 + i] : 0.f;
     }
-    // rows t .. t + 3; left: rows there are (those behind the end have no say, whatever exp makes of 0 x A)
+    // rows t .. t + 3.  whole: all of them, and all states, are there.  Else rows behind the end (left: those there are) leave the states alone, and
+    // states past the last stay 0, whatever exp makes of 0 x A and an infinite x of 0 x B.
     auto four_rows = [&](auto whole, int buf, int t, int left, float *p) {
       const ulonglong2 d4 = *reinterpret_cast<const ulonglong2 *>(&sm.delta[buf][ch_in][t]), u4 = *reinterpret_cast<const ulonglong2 *>(&sm.u[buf][ch_in][t]);
       unsigned long long y01 = 0, y23 = 0;
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float next = fmaf(ex2(e[q]), h[i], w[q]);
-          h[i] = decltype(whole)::value || t + q < left ? next : h[i];
+          h[i] = decltype(whole)::value || (t + q < left && n0 + i < a.n) ? next : h[i];
           hs[q] = h[i];
         }
         if (MODE != SSM_ENDS) {
@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
     for (int k = 0; k < tiles; ++k) {
       const int buf = k & 1;
       pair_sync<SSM_BAR_FULL, FULL_N>(buf);
-      if (k < full) tile(std::true_type{}, buf, SSM_ROWS);
-      else tile(std::false_type{}, buf, (int)(end - row) - full * SSM_ROWS);
+      if (k < full && a.n == NP) tile(std::true_type{}, buf, SSM_ROWS);
+      else tile(std::false_type{}, buf, k < full ? SSM_ROWS : (int)(end - row) - full * SSM_ROWS);
       if (MODE == SSM_ENDS) pair_arrive<SSM_BAR_FREE, FREE_N>(buf);
       else pair_arrive<SSM_BAR_DONE, DONE_N>(buf);
     }
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
       }
       pair_sync<SSM_BAR_IN, SSM_IN>(0);   // everybody's part of tile k is there
       const long long t0 = row + (long long)k * SSM_ROWS;
-Pack<T, 2> x[EACH], dt[EACH];   // (all of them ahead of the first store, which a load would have to stay behind)
+      Pack<T, 2> x[EACH], dt[EACH];   // (all of them ahead of the first store, which a load would have to stay behind)
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int r = row_of(i), c = ch_of(i);
@@ -323,7 +323,7 @@ Pack<T, 2> x[EACH], dt[EACH];   // (all of them ahead of the first store, which 
       const int buf = k & 1;
       const long long t0 = row + (long long)k * SSM_ROWS;
       pair_sync<SSM_BAR_DONE, DONE_N>(buf);
-Pack<T, 2> x[EACH], z[EACH];
+      Pack<T, 2> x[EACH], z[EACH];
       float2 yv[EACH];
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
@@ -340,7 +340,7 @@ Pack<T, 2> x[EACH], z[EACH];
         Pack<T, 2> o;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          y[e] = fmaf(skip[e], to_f(x[i].v[e]), y[e]);
+          if (a.D) y[e] = fmaf(skip[e], to_f(x[i].v[e]), y[e]);
           if (a.z) y[e] *= silu(to_f(z[i].v[e]));
           o.v[e] = from_f<T>(y[e]);
         }

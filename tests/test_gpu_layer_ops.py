@@ -241,6 +241,20 @@ def test_conv_seq(pkg, lengths, taps, d, dtype):
         assert torch.equal(p, new)
 
 
+@pytest.mark.parametrize("d", [1, 5, 75])
+def test_conv_looks_at_no_neighbours(pkg, d):
+    """weights, bias and rows between NaN: a channel count that is no multiple of what a thread takes"""
+    nan = torch.full((4, 4 * d + 64), float("nan"), device="cuda")
+    x, w, b = _rand(20, d, dtype=F16), _rand(d, 4, seed=1), _rand(d, seed=2)
+    nan[0, 16:16 + 4 * d], nan[1, 16:16 + d] = w.flatten(), b
+    wide = torch.full((20, d + 9), float("nan"), dtype=F16, device="cuda")
+    wide[:, 3:3 + d] = x
+    wn, bn, xn = nan[0, 16:16 + 4 * d].view(d, 4), nan[1, 16:16 + d], wide[:, 3:3 + d]
+    assert torch.equal(pkg.conv_seq(xn, wn, bn), pkg.conv_seq(x, w, b))
+    assert torch.equal(pkg.conv_step(xn, wn, bn), pkg.conv_step(x, w, b))
+    assert torch.isfinite(pkg.conv_seq(xn, wn, bn)).all()
+
+
 def test_conv_seq_in_place_states_and_no_states(pkg):
     x, w, b = _rand(50, 64, dtype=F16), _rand(64, 4, seed=1), _rand(64, seed=2)
     starts, pool = [0, 1, 3, 50], _rand(3, 3, 64, dtype=F16, seed=3)
@@ -460,6 +474,25 @@ def test_ssm_extremes(pkg):
     assert torch.isnan(got2[30:, 5]).all()
     rest = [c for c in range(d) if c != 5]
     assert torch.equal(got2[:, rest], got[:, rest]) and torch.equal(got2[:30], got[:30])
+
+
+@pytest.mark.parametrize("d,n,dtype", [(24, 5, F16), (13, 5, F32), (16, 16, F16), (10, 3, BF16), (40, 70, F32)])
+def test_ssm_infinite_inputs(pkg, d, n, dtype):
+    """an infinite x makes its channel infinite, as the formula does: what fills up the lanes behind the last state adds no 0 x inf"""
+    rows = 40
+    x, dt, A, B, C, D, z, bias = _ssm_inputs(rows, d, n, 1, dtype)
+    x, B, C = x.clone(), B.abs().contiguous(), C.abs().contiguous()
+    x[7, 4], x[39, 6] = float("inf"), float("-inf")
+    pool = torch.zeros((rows, d, n), device="cuda")
+    y, ey, new, _ = _ssm_want(x, dt, A, B, C, None, z, bias, True, [0, rows], pool[:1], [-1], [0])
+    assert torch.isinf(y[7:, 4]).all() and torch.isinf(y[39, 6])
+    p = pool[:1].clone()
+    _check(pkg.ssm_seq(x, dt, A, B, C, z=z, dt_bias=bias, state=p, from_slots=-1), y, ey)
+    assert torch.equal(torch.isinf(p), torch.isinf(new)) and not torch.isnan(p).any()
+    y, ey, new, _ = _ssm_want(x, dt, A, B, C, None, z, bias, True, list(range(rows + 1)), pool, list(range(rows)), list(range(rows)))
+    p = pool.clone()
+    _check(pkg.ssm_step(x, dt, A, B, C, z=z, dt_bias=bias, state=p), y, ey)
+    assert torch.equal(torch.isinf(p), torch.isinf(new)) and not torch.isnan(p).any()
 
 
 # ---- slots -------------------------------------------------------------------------------------------------------
