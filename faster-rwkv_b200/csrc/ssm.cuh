@@ -21,20 +21,19 @@ template <typename T> cudaError_t launch_ssm_seq(const SsmArgs &a, const SeqTabl
 
 #ifdef FRB_SSM_KERNELS
 
-// A CTA walks 128 / L channels along the rows of a piece, SSM_ROWS at a time, with three kinds of warps, each at a tile of its own:
+// A CTA walks 128 / L channels along the rows of a piece, SSM_ROWS at a time, with two kinds of warps, each at a tile of its own:
 //   four hold the states, a lane NS of one channel, L lanes a channel;
-//   two bring the next rows in (copies two tiles ahead) and put down what the states need of them: time steps and their products with x, once
-//   per row and channel, B and C in fp32;
-//   two finish the rows behind: skip, gate, rounding, store.
+//   four bring the next rows in (copies two tiles ahead) and put down what the states need of them (time steps and their products with x, once per
+//   row and channel, B and C in fp32), and finish the rows behind: skip, gate, rounding, store.
 // (One warp that does all of it took four times as long for a row of its own: its chains of dependent instructions follow one another.)
 // Everything lies in shared memory along the rows: a lane takes four rows of a state with loads of 16 bytes, packed products of neighbouring rows and
 // one multiply-add a row.  The sums over a channel's lanes are taken L rows at a time, so that every lane ends with one row's (L - 1
 // shuffles for L rows).
-// What bounds it: with work for all SMs the words that lanes load from shared memory, 2 L + 32 a row of 32 channels (16 states), next
-// to 40 clocks of exponentials; alone, a warp's own latency, 42 clocks a row with one state a lane, 65 with two, 85 with four.
+// What bounds it: with work for all SMs the words that lanes load from shared memory, 2 L + 32 a row of 32 channels (16 states), next to 40
+// clocks of exponentials; alone, the two state warps a scheduler has at most: half of the time they wait for their own results.
 //   SSM_WHOLE: the piece is the sequence      SSM_ENDS: the piece's state from zero, and the sum of its time steps
 //   SSM_PIECE: the piece from the state that the pieces before it leave
-constexpr int SSM_ROWS = 32, SSM_STATES = 128, SSM_IN = 64, SSM_OUT = 64, SSM_THREADS = SSM_STATES + SSM_IN + SSM_OUT, SSM_RING = 4;
+constexpr int SSM_ROWS = 32, SSM_STATES = 128, SSM_HELP = 128, SSM_THREADS = SSM_STATES + SSM_HELP, SSM_RING = 4;
 constexpr int SSM_LD = SSM_ROWS + 4;   // 16 bytes more than the rows: eight lanes' loads meet in no bank
 enum { SSM_WHOLE = 0, SSM_ENDS = 1, SSM_PIECE = 2 };
 template <typename T, int NS, int L>
@@ -46,8 +45,8 @@ struct SsmTile {
   static __device__ __forceinline__ int bc_at(int n) { return n % NS * L + n / NS; }
   float y[2][SSM_ROWS][YS];
 };
-// named barriers, two of each: rows put down; states done with them; rows finished (their buffers are free)
-enum { SSM_BAR_FULL = 1, SSM_BAR_DONE = 3, SSM_BAR_FREE = 5, SSM_BAR_IN = 7 };
+// named barriers: rows put down and states done with them (two of each); the helpers among themselves
+enum { SSM_BAR_FULL = 1, SSM_BAR_DONE = 3, SSM_BAR_HELP = 5 };
 template <int ID, int N> __device__ __forceinline__ void pair_sync(int which) { if (which) asm volatile("bar.sync %0, %1;" ::"n"(ID + 1), "n"(N) : "memory"); else asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
 template <int ID, int N> __device__ __forceinline__ void pair_arrive(int which) { if (which) asm volatile("bar.arrive %0, %1;" ::"n"(ID + 1), "n"(N) : "memory"); else asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
 __device__ __forceinline__ void copy_async16(void *dst, const void *src) {
@@ -63,7 +62,6 @@ template <typename T, int NS, int L, int CTAS, int MODE, bool VEC>
 __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
   using Tile = SsmTile<T, NS, L>;
   constexpr int CH = Tile::CH, NP = Tile::NP;
-  constexpr int FULL_N = SSM_STATES + SSM_IN, DONE_N = SSM_STATES + SSM_OUT, FREE_N = SSM_IN + (MODE == SSM_ENDS ? SSM_STATES : SSM_OUT);
   extern __shared__ __align__(16) uint8_t ssm_smem[];
   Tile &sm = *reinterpret_cast<Tile *>(ssm_smem);
   int s, piece = 0;
@@ -132,12 +130,14 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
       p[0] = p01.x; p[1] = p01.y; p[2] = p23.x; p[3] = p23.y;
     };
     auto tile = [&](auto whole, int buf, int left) {
-      constexpr int STEP = L > 8 ? L : 8;
+      constexpr int STEP = NS > 2 ? (L > 8 ? L : 8) : (L < 8 ? 4 * L : SSM_ROWS);   // rows whose sums over the lanes are taken at a time
 #pragma unroll 1
       for (int t0 = 0; t0 < (decltype(whole)::value ? SSM_ROWS : left); t0 += STEP) {
         float p[STEP];
 #pragma unroll
-        for (int r = 0; r < STEP; r += 4) four_rows(whole, buf, t0 + r, left, p + r);
+        for (int r = 0; r < STEP; r += 4) {
+          four_rows(whole, buf, t0 + r, left, p + r);
+        }
         if (MODE != SSM_ENDS)
           // L rows' parts -> every lane the sum of one of them
 #pragma unroll
@@ -157,11 +157,10 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
     };
     for (int k = 0; k < tiles; ++k) {
       const int buf = k & 1;
-      pair_sync<SSM_BAR_FULL, FULL_N>(buf);
+      pair_sync<SSM_BAR_FULL, SSM_THREADS>(buf);
       if (k < full && a.n == NP) tile(std::true_type{}, buf, SSM_ROWS);
       else tile(std::false_type{}, buf, k < full ? SSM_ROWS : (int)(end - row) - full * SSM_ROWS);
-      if (MODE == SSM_ENDS) pair_arrive<SSM_BAR_FREE, FREE_N>(buf);
-      else pair_arrive<SSM_BAR_DONE, DONE_N>(buf);
+      pair_arrive<SSM_BAR_DONE, SSM_THREADS>(buf);
     }
     float *to = nullptr;
     if (MODE == SSM_ENDS) to = work;
@@ -173,169 +172,146 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
     return;
   }
 
-  const int ch_left = ch_end - ch0;   // channels of the tile that there are
-  if (threadIdx.x < SSM_STATES + SSM_IN) {
-    // ---- rows in ----
-    // a thread's places in a tile: a warp takes eight rows of eight channels at a time (four lanes, two channels each), in which neither its loads
-    // along the channels nor its stores along the rows meet in a bank
-    const int tid = threadIdx.x - SSM_STATES, sub = tid & 3;
-    constexpr int BLOCKS = CH / 8, EACH = BLOCKS * 2, ARRAYS = MODE == SSM_ENDS ? 2 : 3;   // (two warps, 16 rows each)
-    auto row_of = [&](int i) { return tid / 32 * 16 + i / BLOCKS * 8 + (tid & 31) / 4; };
-    auto ch_of = [&](int i) { return i % BLOCKS * 8 + sub * 2; };
-    float bias[BLOCKS][2], dsum[BLOCKS][2];
+  // ---- rows in, rows out ----
+  const int tid = threadIdx.x - SSM_STATES, ch_left = ch_end - ch0;   // channels of the tile that there are
+  // Time steps: a warp takes eight rows, eight channels of them at a time (four lanes a row, two channels each), in which neither its loads
+  // along the channels nor its stores along the rows meet in a bank.
+  constexpr int BLOCKS = CH / 8, ARRAYS = MODE == SSM_ENDS ? 2 : 3;
+  const int in_row = tid / 4, in_ch = (tid & 3) * 2;
+  float bias[BLOCKS][2], dsum[BLOCKS][2];
 #pragma unroll
-    for (int g = 0; g < BLOCKS; ++g)
+  for (int g = 0; g < BLOCKS; ++g)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        bias[g][e] = a.dt_bias && ch_of(g) + e < ch_left ? a.dt_bias[ch0 + ch_of(g) + e] : 0.f;
-        dsum[g][e] = 0.f;
-      }
-    const T *src[3] = {reinterpret_cast<const T *>(a.x) + ch0, reinterpret_cast<const T *>(a.dt) + ch0, reinterpret_cast<const T *>(a.z ? a.z : a.x) + ch0};
-    const long long ld[3] = {a.ldx, a.lddt, a.z ? a.ldz : a.ldx};
-    // Rows and channels past the end repeat the last (and count for nothing): a load that is made or not is waited for where its ways meet.
-    constexpr int UNIT = 16 / (int)sizeof(T), ROW_UNITS = CH / UNIT, COPIES = SSM_ROWS * ROW_UNITS, PER = (COPIES + SSM_IN - 1) / SSM_IN;
-    constexpr int SINGLE = SSM_ROWS * CH / SSM_IN;
-    T hold[VEC ? 1 : 3 * SINGLE];
-    auto ask = [&](int k) {   // tile k: copies into its place in the ring, or (not VEC) elements into registers
-      const long long t0 = row + (long long)k * SSM_ROWS;
-      const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
-#pragma unroll
-      for (int arr = 0; arr < ARRAYS; ++arr) {
-        if constexpr (VEC) {
-#pragma unroll
-          for (int q = 0; q < PER; ++q) {
-            const int e = tid + q * SSM_IN, r = e / ROW_UNITS, c = e % ROW_UNITS * UNIT;
-            if (e < COPIES) copy_async16(&sm.in[k % SSM_RING][arr][r][c], src[arr] + (t0 + min(r, final_row)) * ld[arr] + min(c, (ch_left - 1) / UNIT * UNIT));
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < SINGLE; ++q) {
-            const int e = tid + q * SSM_IN;
-            hold[arr * SINGLE + q] = src[arr][(t0 + min(e / CH, final_row)) * ld[arr] + min(e % CH, ch_left - 1)];
-          }
-        }
-      }
-      if (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    auto keep = [&](int k) {
-      if constexpr (!VEC) {
-#pragma unroll
-        for (int arr = 0; arr < ARRAYS; ++arr)
-#pragma unroll
-          for (int q = 0; q < SINGLE; ++q) sm.in[k % SSM_RING][arr][(tid + q * SSM_IN) / CH][(tid + q * SSM_IN) % CH] = hold[arr * SINGLE + q];
-      }
-    };
-    // B and C: one column, every BROWS-th row (or all rows of several columns); columns past the last are 0
-    constexpr int BROWS = SSM_IN >= NP ? SSM_IN / NP : 1, BCOLS = SSM_IN >= NP ? 1 : NP / SSM_IN, BPT = SSM_ROWS / BROWS * BCOLS, BATCH = BPT < 16 ? BPT : 16;
-    const int bcol = tid % NP, brow = tid / NP;
-    const T *bp = reinterpret_cast<const T *>(a.B) + (long long)group * a.n, *cp = reinterpret_cast<const T *>(a.C) + (long long)group * a.n;
-    T bn[BATCH], cn[BATCH];
-    auto bc_ask = [&](int k, int q0) {
-      const long long t0 = row + (long long)k * SSM_ROWS;
-      const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
-      const T *b = bp + t0 * a.ldb, *c = cp + t0 * a.ldc;
-#pragma unroll
-      for (int q = 0; q < BATCH; ++q) {
-        const int r = min(brow + (q0 + q) / BCOLS * BROWS, final_row), col = min(bcol + (q0 + q) % BCOLS * SSM_IN, a.n - 1);
-        bn[q] = b[r * a.ldb + col];
-        if (MODE != SSM_ENDS) cn[q] = c[r * a.ldc + col];
-      }
-    };
-    auto bc_put = [&](int buf, int q0) {
-#pragma unroll
-      for (int q = 0; q < BATCH; ++q) {
-        const int r = brow + (q0 + q) / BCOLS * BROWS, col = bcol + (q0 + q) % BCOLS * SSM_IN;
-        sm.b[buf][Tile::bc_at(col)][r] = col < a.n ? to_f(bn[q]) : 0.f;
-        if (MODE != SSM_ENDS) sm.c[buf][Tile::bc_at(col)][r] = col < a.n ? to_f(cn[q]) : 0.f;
-      }
-    };
-    if (tiles > 0) {
-      ask(0);
-      if (VEC) ask(1);   // (past the end too: the last row again)
-      bc_ask(0, 0);
+    for (int e = 0; e < 2; ++e) {
+      bias[g][e] = a.dt_bias && g * 8 + in_ch + e < ch_left ? a.dt_bias[ch0 + g * 8 + in_ch + e] : 0.f;
+      dsum[g][e] = 0.f;
     }
-    for (int k = 0; k < tiles; ++k) {
-      const int buf = k & 1;
-      if (k >= 2) pair_sync<SSM_BAR_FREE, FREE_N>(buf);   // tile k - 2 is finished
-      if (VEC) {
-        ask(k + 2);
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
+  const T *src[3] = {reinterpret_cast<const T *>(a.x) + ch0, reinterpret_cast<const T *>(a.dt) + ch0, reinterpret_cast<const T *>(a.z ? a.z : a.x) + ch0};
+  const long long ld[3] = {a.ldx, a.lddt, a.z ? a.ldz : a.ldx};
+  // Rows and channels past the end repeat the last (and count for nothing): a load that is made or not is waited for where its ways meet.
+  constexpr int UNIT = 16 / (int)sizeof(T), ROW_UNITS = CH / UNIT, COPIES = SSM_ROWS * ROW_UNITS, PER = (COPIES + SSM_HELP - 1) / SSM_HELP;
+  constexpr int SINGLE = SSM_ROWS * CH / SSM_HELP;
+  T hold[VEC ? 1 : 3 * SINGLE];
+  auto ask = [&](int k) {   // tile k: copies into its place in the ring, or (not VEC) elements into registers
+    const long long t0 = row + (long long)k * SSM_ROWS;
+    const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
+#pragma unroll
+    for (int arr = 0; arr < ARRAYS; ++arr) {
+      if constexpr (VEC) {
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+          const int e = tid + q * SSM_HELP, r = e / ROW_UNITS, c = e % ROW_UNITS * UNIT;
+          if (e < COPIES) copy_async16(&sm.in[k % SSM_RING][arr][r][c], src[arr] + (t0 + min(r, final_row)) * ld[arr] + min(c, (ch_left - 1) / UNIT * UNIT));
+        }
       } else {
-        keep(k);
-        ask(k + 1);
-      }
-      pair_sync<SSM_BAR_IN, SSM_IN>(0);   // everybody's part of tile k is there
-      const long long t0 = row + (long long)k * SSM_ROWS;
-      Pack<T, 2> x[EACH], dt[EACH];   // (all of them ahead of the first store, which a load would have to stay behind)
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int r = row_of(i), c = ch_of(i);
-        x[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][0][r][c]);
-        dt[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][1][r][c]);
-      }
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int r = row_of(i), c = ch_of(i);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = to_f(dt[i].v[e]) + bias[i % BLOCKS][e];
-          if (a.softplus) v = softplus(v);
-          if (MODE == SSM_ENDS && t0 + r < end) dsum[i % BLOCKS][e] += v;
-          sm.delta[buf][c + e][r] = v;
-          sm.u[buf][c + e][r] = v * to_f(x[i].v[e]);
+        for (int q = 0; q < SINGLE; ++q) {
+          const int e = tid + q * SSM_HELP;
+          hold[arr * SINGLE + q] = src[arr][(t0 + min(e / CH, final_row)) * ld[arr] + min(e % CH, ch_left - 1)];
         }
       }
-      bc_put(buf, 0);
-      for (int q0 = BATCH; q0 < BPT; q0 += BATCH) { bc_ask(k, q0); bc_put(buf, q0); }
-      bc_ask(k + 1, 0);
-      pair_arrive<SSM_BAR_FULL, FULL_N>(buf);
     }
-    if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (tiles > 1) pair_sync<SSM_BAR_FREE, FREE_N>(tiles & 1);
-    if (tiles > 0) pair_sync<SSM_BAR_FREE, FREE_N>((tiles - 1) & 1);
-    if (MODE == SSM_ENDS) {
-      // the sum of a channel's time steps, over the rows' threads in a fixed order (the buffers are free)
+    if (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto keep = [&](int k) {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int arr = 0; arr < ARRAYS; ++arr)
+#pragma unroll
+        for (int q = 0; q < SINGLE; ++q) sm.in[k % SSM_RING][arr][(tid + q * SSM_HELP) / CH][(tid + q * SSM_HELP) % CH] = hold[arr * SINGLE + q];
+    }
+  };
+  // B and C: four rows of a column at a time; columns past the last are 0
+  constexpr int FOURS = NP * (SSM_ROWS / 4), EACH4 = (FOURS + SSM_HELP - 1) / SSM_HELP, BATCH = EACH4 < 2 ? EACH4 : 2;
+  const T *bp = reinterpret_cast<const T *>(a.B) + (long long)group * a.n, *cp = reinterpret_cast<const T *>(a.C) + (long long)group * a.n;
+  struct { T b[4], c[4]; } bc[BATCH];
+  auto bc_ask = [&](int k, int q0) {
+    const long long t0 = row + (long long)k * SSM_ROWS;
+    const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
+    const T *b = bp + t0 * a.ldb, *c = cp + t0 * a.ldc;
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int e = tid + (q0 + q) * SSM_HELP, col = min(e % NP, a.n - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = min(e / NP * 4 + i, final_row);
+        bc[q].b[i] = b[r * a.ldb + col];
+        if (MODE != SSM_ENDS) bc[q].c[i] = c[r * a.ldc + col];
+      }
+    }
+  };
+  auto bc_put = [&](int buf, int q0) {
+#pragma unroll
+    for (int q = 0; q < BATCH; ++q) {
+      const int e = tid + (q0 + q) * SSM_HELP, col = e % NP;
+      if (e < FOURS) {
+        float4 b, c;
+        b.x = to_f(bc[q].b[0]); b.y = to_f(bc[q].b[1]); b.z = to_f(bc[q].b[2]); b.w = to_f(bc[q].b[3]);
+        *reinterpret_cast<float4 *>(&sm.b[buf][Tile::bc_at(col)][e / NP * 4]) = col < a.n ? b : float4{};
+        if (MODE != SSM_ENDS) {
+          c.x = to_f(bc[q].c[0]); c.y = to_f(bc[q].c[1]); c.z = to_f(bc[q].c[2]); c.w = to_f(bc[q].c[3]);
+          *reinterpret_cast<float4 *>(&sm.c[buf][Tile::bc_at(col)][e / NP * 4]) = col < a.n ? c : float4{};
+        }
+      }
+    }
+  };
+  // rows out: two channels of every STRIDE-th row
+  constexpr int CP = CH / 2, STRIDE = SSM_HELP / CP, EACH = SSM_ROWS / STRIDE;
+  const int out_ch = tid % CP * 2, out_row = tid / CP;
+  float skip[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) skip[i] = a.D && out_ch + i < ch_left ? a.D[ch0 + out_ch + i] : 0.f;
+  T *op = reinterpret_cast<T *>(a.out) + ch0 + out_ch;
+  if (tiles > 0) {
+    ask(0);
+    if (VEC) ask(1);   // (past the end too: the last row again)
+    bc_ask(0, 0);
+  }
+  for (int k = 0; k <= tiles; ++k) {
+    const int buf = k & 1;
+    if (k < tiles) {
+      if (VEC) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else keep(k);
+      pair_sync<SSM_BAR_HELP, SSM_HELP>(0);   // everybody's part of tile k is there, and nobody is at tile k - 2 any more
+      ask(k + (VEC ? 2 : 1));
+      const long long t0 = row + (long long)k * SSM_ROWS;
+      Pack<T, 2> x[BLOCKS], dt[BLOCKS];   // (all of them ahead of the first store, which a load would have to stay behind)
+#pragma unroll
+      for (int g = 0; g < BLOCKS; ++g) {
+        x[g] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][0][in_row][g * 8 + in_ch]);
+        dt[g] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][1][in_row][g * 8 + in_ch]);
+      }
 #pragma unroll
       for (int g = 0; g < BLOCKS; ++g)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) sm.y[0][tid / 4][ch_of(g) + e] = dsum[g][e];
-      pair_sync<SSM_BAR_IN, SSM_IN>(0);
-      for (int c = tid; c < CH && c < ch_left; c += SSM_IN) {
-        float v = 0.f;
-        for (int r = 0; r < SSM_IN / 4; ++r) v += sm.y[0][r][c];
-        work[dn + ch0 + c] = v;
-      }
+        for (int e = 0; e < 2; ++e) {
+          float v = to_f(dt[g].v[e]) + bias[g][e];
+          if (a.softplus) v = softplus(v);
+          if (MODE == SSM_ENDS && t0 + in_row < end) dsum[g][e] += v;
+          sm.delta[buf][g * 8 + in_ch + e][in_row] = v;
+          sm.u[buf][g * 8 + in_ch + e][in_row] = v * to_f(x[g].v[e]);
+        }
+      bc_put(buf, 0);
+      for (int q0 = BATCH; q0 < EACH4; q0 += BATCH) { bc_ask(k, q0); bc_put(buf, q0); }
+      bc_ask(k + 1, 0);
+      pair_arrive<SSM_BAR_FULL, SSM_THREADS>(buf);
     }
-    return;
-  }
-
-  // ---- rows out ----
-  if constexpr (MODE != SSM_ENDS) {
-    // a thread's places: two channels of every STRIDE-th row
-    constexpr int CP = CH / 2;   // (up to 64 threads)
-    const int tid = threadIdx.x - SSM_STATES - SSM_IN, cc = tid % CP * 2, r0 = tid / CP;
-    constexpr int STRIDE = SSM_OUT / CP, EACH = SSM_ROWS / STRIDE;
-    float skip[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) skip[i] = a.D && cc + i < ch_left ? a.D[ch0 + cc + i] : 0.f;
-    T *op = reinterpret_cast<T *>(a.out) + ch0 + cc;
-    for (int k = 0; k < tiles; ++k) {
-      const int buf = k & 1;
-      const long long t0 = row + (long long)k * SSM_ROWS;
-      pair_sync<SSM_BAR_DONE, DONE_N>(buf);
+    if (k == 0) continue;
+    pair_sync<SSM_BAR_DONE, SSM_THREADS>(buf ^ 1);   // the states are behind tile k - 1: its rows go out, its buffers are tile k + 1's
+    if constexpr (MODE != SSM_ENDS) {
+      const long long t0 = row + (long long)(k - 1) * SSM_ROWS;
       Pack<T, 2> x[EACH], z[EACH];
       float2 yv[EACH];
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
-        const int r = r0 + i * STRIDE;
-        x[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][0][r][cc]);
-        z[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[k % SSM_RING][2][r][cc]);
-        yv[i] = *reinterpret_cast<const float2 *>(&sm.y[buf][r][cc]);
+        const int r = out_row + i * STRIDE;
+        x[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[(k - 1) % SSM_RING][0][r][out_ch]);
+        z[i] = *reinterpret_cast<const Pack<T, 2> *>(&sm.in[(k - 1) % SSM_RING][2][r][out_ch]);
+        yv[i] = *reinterpret_cast<const float2 *>(&sm.y[buf ^ 1][r][out_ch]);
       }
-      pair_arrive<SSM_BAR_FREE, FREE_N>(buf);
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
-        const int r = r0 + i * STRIDE;
+        const int r = out_row + i * STRIDE;
         float y[2] = {yv[i].x, yv[i].y};
         Pack<T, 2> o;
 #pragma unroll
@@ -344,8 +320,22 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
           if (a.z) y[e] *= silu(to_f(z[i].v[e]));
           o.v[e] = from_f<T>(y[e]);
         }
-        if (t0 + r < end && cc < ch_left) store_pack<T, 2, VEC>(op + (t0 + r) * a.ldo, o, ch_left - cc);
+        if (t0 + r < end && out_ch < ch_left) store_pack<T, 2, VEC>(op + (t0 + r) * a.ldo, o, ch_left - out_ch);
       }
+    }
+  }
+  if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (MODE == SSM_ENDS) {
+    // the sum of a channel's time steps, over the rows' threads in a fixed order
+#pragma unroll
+    for (int g = 0; g < BLOCKS; ++g)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sm.y[0][in_row][g * 8 + in_ch + e] = dsum[g][e];
+    pair_sync<SSM_BAR_HELP, SSM_HELP>(0);
+    if (tid < CH && tid < ch_left) {
+      float v = 0.f;
+      for (int r = 0; r < SSM_ROWS; ++r) v += sm.y[0][r][tid];
+      work[dn + ch0 + tid] = v;
     }
   }
 }
@@ -397,34 +387,35 @@ cudaError_t ssm_seq_split(const SsmArgs &a, const SeqTable &t, cudaStream_t st) 
   if (e == cudaSuccess) e = op_launch(ssm_join_kernel, dim3((unsigned)(((size_t)a.d * a.n + 255) / 256), t.n), 256, 0, st, 1, a, t);
   return e == cudaSuccess ? ssm_seq_mode<T, NS, L, 2, SSM_PIECE, VEC>(a, t, items, st) : e;
 }
-// States a lane.  Few channels and sequences: fewer states, more CTAs and the shorter chain, as long as every CTA has an SM (4096 rows of 768
-// channels with 16 states: 92 us with one a lane, 141 with two, 184 with four; of 1536: 136, 141, 184; of 2560: 219, 205, 185).  Many:
-// three CTAs an SM where their registers allow it (11 sequences of 5120 channels 118 us against 131; one of 4096 230 against 186).
+// States a lane.  Few channels and sequences: fewer states, more CTAs and the shorter chain (4096 rows of 768 channels with 16 states: 79 us with one a
+// lane, 106 with two, 183 with four; of 1536: 121, 106, 183; of 4096: 251, 171, 186; two sequences of 4096: 251, 170, 145; 1000 rows of
+// 2048 with 64: 84 with four a lane, 93 with eight; 4096 of 4096 with 8: 149 with one, 163 with two).  Many: three CTAs an SM where
+// their registers allow it (11 sequences of 5120 channels 117 us against 128; one of 4096 190 against 186).
 template <typename T, bool VEC>
 cudaError_t ssm_seq_any(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {
   auto ctas = [&](int ch) { return (long long)((a.d / a.groups + ch - 1) / ch) * a.groups * t.n; };
   const int sms = device_sm_count();
   if (a.n <= 8) {
     if (a.shift) return ssm_seq_split<T, 2, 4, VEC>(a, t, st);
-    if (ctas(16) <= sms) return ssm_seq_mode<T, 1, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(16) <= 2 * sms) return ssm_seq_mode<T, 1, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     if (ctas(32) <= 2 * sms) return ssm_seq_mode<T, 2, 4, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     return ssm_seq_mode<T, 2, 4, 3, SSM_WHOLE, VEC>(a, t, t.n, st);
   }
   if (a.n <= 16) {
     if (a.shift) return ssm_seq_split<T, 4, 4, VEC>(a, t, st);
     if (ctas(8) <= sms) return ssm_seq_mode<T, 1, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
-    if (ctas(16) <= sms) return ssm_seq_mode<T, 2, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(16) <= 2 * sms) return ssm_seq_mode<T, 2, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     if (ctas(32) <= 2 * sms) return ssm_seq_mode<T, 4, 4, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     return ssm_seq_mode<T, 4, 4, 3, SSM_WHOLE, VEC>(a, t, t.n, st);
   }
   if (a.n <= 32) {
     if (a.shift) return ssm_seq_split<T, 4, 8, VEC>(a, t, st);
-    if (ctas(8) <= sms) return ssm_seq_mode<T, 2, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(8) <= 2 * sms) return ssm_seq_mode<T, 2, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     return ssm_seq_mode<T, 4, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
   }
   if (a.n <= 64) {
     if (a.shift) return ssm_seq_split<T, 8, 8, VEC>(a, t, st);
-    if (ctas(8) <= sms) return ssm_seq_mode<T, 4, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(8) <= 2 * sms) return ssm_seq_mode<T, 4, 16, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     return ssm_seq_mode<T, 8, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
   }
   if (a.shift) return ssm_seq_split<T, 8, 16, VEC>(a, t, st);
