@@ -79,6 +79,8 @@ void fill_slots(SlotTable &t, int i0, int n, const void *state, const int32_t *f
 
 // ---- the short causal convolution --------------------------------------------------------------------------------
 // y[t, d] = act(b[d] + sum_j w[d, j] x[t - (W - 1) + j, d]); what lies before a sequence's first row are the W - 1 rows of its state.
+// Bound by memory: x once, y once, for a few multiply-adds an element.  4001 rows of 5120 bf16 channels in 37 sequences, 82 MB: 24 us, 3.4 TB/s (a
+// copy of the same rows with torch 46); 8 rows a thread 27, 8 channels a thread 31.  One token of 64 streams of 4096 channels 2.5 us.
 struct ConvArgs {
   const void *x;
   void *out, *state;
@@ -265,7 +267,7 @@ int conv_check(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const
 // One token of each stream.  L lanes share CPT neighbouring channels, four states of each a lane (and every 4 L-th four): their states are all asked for
 // at once.  Each of the first CPT lanes brings x, dt and z of one channel, makes its time step for the others, and ends with its sum over
 // the states.  Bound by reading and writing the states: 256 streams of 4096 channels with 16 states 134 MB; with x, dt, z and the time
-// step made by every lane it was bound by 708 instructions a warp.
+// step made by every lane it was bound by 708 instructions a warp.  31 us so, 4.3 TB/s; one stream of 5120 channels 2.3 us.
 template <typename T, int L, bool VEC>
 __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const __grid_constant__ SlotTable tab) {
   constexpr int CPT = L < 4 ? L : 4, CH = 128 / L * CPT;
@@ -406,7 +408,8 @@ int ssm_split(int64_t rows, int n_seq, int d) {
 // slot of the call to itself: it brings those of the sources into shared memory, then writes them to the slots that take them.  Both
 // sides go by the 16-byte words of memory; where slots begin between them (GRAN < 16: the granule they all are multiples of), a
 // source's words lie in shared memory as they lay, and a word to be written is cut out of two of them.
-// Bound by the bytes: every source once, every destination once.
+// Bound by the bytes: every source once, every destination once.  256 slots of 2.1 MB in a new order that leaves
+// some out: 162 us, 5.4 TB/s; 31 copies of one of 389 KB 4.
 constexpr int COPY_CAP = 4096, COPY_SMALL = 64, COPY_THREADS = 256, COPY_SMEM = 96 * 1024;
 template <int CAP>
 struct CopyTable {
