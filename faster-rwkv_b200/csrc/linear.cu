@@ -413,6 +413,12 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
   }
   tc_fence_before();
   __syncthreads();
+  // The tensor memory goes back before the CTA waits for the others of its cluster: held until they are done, it could be what one of them waits for,
+  // by way of a third kernel's CTAs that hold the rest.
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  }
   if (p.split > 1) cluster_sync();
   // a warp finishes a row: four channels a lane.  Rows of the cluster's CTAs in turn.
   const int n = ch0 + lane * 4;
@@ -453,7 +459,6 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
     }
   }
   if (p.split > 1) cluster_sync();   // nobody leaves while its sums are read
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
 // Many rows: out[256 rows, bn channels] per pair of SMs (tcgen05.mma.cta_group::2, bn up to 256), one CTA on each SM that walks tile after tile with

@@ -166,6 +166,29 @@ def test_linear_is_the_same_every_time_and_on_any_stream(pkg):
         assert all(torch.equal(first, a) for a in again)
 
 
+def test_calls_on_several_streams_at_once(pkg):
+    """products of every kind, scans and convolutions side by side: what each gives alone"""
+    w, wide = _rand(2560, 2560, dtype=F16, scale=0.02, seed=1), _rand(640, 2560, dtype=F16, scale=0.02, seed=2)
+    xs = [_rand(m, 2560, dtype=F16, seed=m) for m in (8, 40, 70, 150, 250, 700, 1500)]
+    d, n = 320, 16
+    sx, dt, A, B, C, D, z, bias = _ssm_inputs(300, d, n, 1, F16)
+    cw = _rand(d, 4, seed=5)
+    jobs = [lambda i=i: pkg.linear(xs[i], w, activation="silu") for i in range(len(xs))] + [lambda i=i: pkg.linear(xs[i], wide) for i in range(len(xs))]
+    jobs += [lambda: pkg.ssm_seq(sx, dt, A, B, C, D=D, z=z, dt_bias=bias), lambda: pkg.conv_seq(sx, cw)]
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for r in range(12):
+        for s, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                for i in range(s, len(jobs), len(streams)):
+                    got.append((i + r) % len(jobs))
+                    got.append(jobs[(i + r) % len(jobs)]())
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i, y in zip(got[::2], got[1::2]))
+
+
 def test_linear_rows_do_not_depend_on_their_neighbours(pkg):
     x, w = _rand(300, 512, dtype=F16), _rand(264, 512, dtype=F16, scale=0.05, seed=1)
     y = pkg.linear(x, w)
