@@ -79,8 +79,9 @@ void fill_slots(SlotTable &t, int i0, int n, const void *state, const int32_t *f
 
 // ---- the short causal convolution --------------------------------------------------------------------------------
 // y[t, d] = act(b[d] + sum_j w[d, j] x[t - (W - 1) + j, d]); what lies before a sequence's first row are the W - 1 rows of its state.
-// Bound by memory: x once, y once, for a few multiply-adds an element.  4001 rows of 5120 bf16 channels in 37 sequences, 82 MB: 24 us, 3.4 TB/s (a
-// copy of the same rows with torch 46); 8 rows a thread 27, 8 channels a thread 31.  One token of 64 streams of 4096 channels 2.5 us.
+// Bound by memory: x once, y once, for a few multiply-adds an element.  4001 rows of 5120 bf16 channels in 37 sequences, 82 MB: 22 us, 3.7 TB/s (a
+// copy of the same rows with torch 46); 8 rows a thread 27, 8 channels a thread 31.  Loads without a branch: what is not there is read from some
+// place that is, and not taken (24 us with branches).  One token of 64 streams of 4096 channels 2.5 us.
 struct ConvArgs {
   const void *x;
   void *out, *state;
@@ -126,20 +127,20 @@ __global__ void __launch_bounds__(128) conv_seq_kernel(const ConvArgs a, const _
   T *out = reinterpret_cast<T *>(a.out) + c + row0 * a.ldo, *state = reinterpret_cast<T *>(a.state) + c;
   const int from = piece == 0 ? tab.from[s] : 0;
   // what lies before the piece: rows of x, or of the state, or zeros
-  const T *back = piece > 0 ? xr - (W - 1) * a.ldx : state + (long long)max(from, 0) * a.state_stride;
-  const long long back_ld = piece > 0 ? a.ldx : a.D;
   const bool zeros = piece == 0 && from < 0;
+  const T *spare = reinterpret_cast<const T *>(a.w) + c;   // (W rows of D fp32: something that is there, and not taken)
+  const T *back = piece > 0 ? xr - (W - 1) * a.ldx : zeros ? spare : state + (long long)from * a.state_stride, *rows_in = rows > 0 ? xr : spare;
+  const long long back_ld = piece > 0 ? a.ldx : a.D;
   Pack<T, V> before[W - 1], in[CONV_ROWS];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) before[j] = load_pack<T, V, VEC>(back + j * back_ld, n);
+#pragma unroll
+  for (int r = 0; r < CONV_ROWS; ++r) in[r] = load_pack<T, V, VEC>(rows_in + (long long)max(min(r, rows - 1), 0) * a.ldx, n);
 #pragma unroll
   for (int j = 0; j < W - 1; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) before[j].v[i] = from_f<T>(0.f);
-  if (!zeros)
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) before[j] = load_pack<T, V, VEC>(back + j * back_ld, n);
-  if (rows > 0)
-#pragma unroll
-    for (int r = 0; r < CONV_ROWS; ++r) in[r] = load_pack<T, V, VEC>(xr + (long long)min(r, rows - 1) * a.ldx, n);
+    for (int i = 0; i < V; ++i)
+      if (zeros) before[j].v[i] = from_f<T>(0.f);
   ConvTaps<W, V, VEC> taps;
   taps.load(a, c, n);
   if (piece == 0 && tab.to[s] >= 0) {
@@ -267,7 +268,8 @@ int conv_check(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const
 // One token of each stream.  L lanes share CPT neighbouring channels, four states of each a lane (and every 4 L-th four): their states are all asked for
 // at once.  Each of the first CPT lanes brings x, dt and z of one channel, makes its time step for the others, and ends with its sum over
 // the states.  Bound by reading and writing the states: 256 streams of 4096 channels with 16 states 134 MB; with x, dt, z and the time
-// step made by every lane it was bound by 708 instructions a warp.  31 us so, 4.3 TB/s; one stream of 5120 channels 2.3 us.
+// step made by every lane it was bound by 708 instructions a warp.  28.5 us so, 4.7 TB/s, with
+// nothing converted ahead of the last load (31 otherwise); one stream of 5120 channels 2.3 us.
 template <typename T, int L, bool VEC>
 __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const __grid_constant__ SlotTable tab) {
   constexpr int CPT = L < 4 ? L : 4, CH = 128 / L * CPT;
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
   const int from_slot = tab.from[s], to_slot = tab.to[s];
   pdl_wait();
   pdl_trigger();
-  const float *from = a.state + (long long)max(from_slot, 0) * a.state_stride;
+  const float *from = from_slot >= 0 ? a.state + (long long)from_slot * a.state_stride : a.A;   // (none: something that is there, and not taken)
   float *to = a.state + (long long)max(to_slot, 0) * a.state_stride;
   const T *bp = reinterpret_cast<const T *>(a.B) + row * a.ldb + (long long)group * a.n;
   const T *cp = reinterpret_cast<const T *>(a.C) + row * a.ldc + (long long)group * a.n;
@@ -287,8 +289,8 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
 #pragma unroll
   for (int k = 0; k < CPT; ++k) at[k] = min(ch0 + k, ch_end - 1) * a.n;
   const int mine = min(ch0 + lane % CPT, ch_end - 1);
-  const float x = to_f(reinterpret_cast<const T *>(a.x)[row * a.ldx + mine]), dt = to_f(reinterpret_cast<const T *>(a.dt)[row * a.lddt + mine]);
-  const float z = a.z ? to_f(reinterpret_cast<const T *>(a.z)[row * a.ldz + mine]) : 0.f;
+  const T x = reinterpret_cast<const T *>(a.x)[row * a.ldx + mine], dt = reinterpret_cast<const T *>(a.dt)[row * a.lddt + mine];
+  const T z = a.z ? reinterpret_cast<const T *>(a.z)[row * a.ldz + mine] : from_f<T>(0.f);
   const float bias = a.dt_bias ? a.dt_bias[mine] : 0.f, skip = a.D ? a.D[mine] : 0.f;
   float delta = 0.f, u = 0.f, y[CPT];
 #pragma unroll
@@ -297,19 +299,14 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
     const int n = n0 + lane * 4, there = a.n - n, left = VEC ? 4 : min(max(there, 1), 4), nc = VEC ? min(n, a.n - 4) : min(n, a.n - 1);
     Pack<float, 4> h[CPT], A4[CPT];
 #pragma unroll
-    for (int k = 0; k < CPT; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[k].v[i] = 0.f;
-    if (from_slot >= 0)
-#pragma unroll
-      for (int k = 0; k < CPT; ++k) h[k] = load_pack<float, 4, VEC>(from + at[k] + nc, left);
+    for (int k = 0; k < CPT; ++k) h[k] = load_pack<float, 4, VEC>(from + at[k] + nc, left);
 #pragma unroll
     for (int k = 0; k < CPT; ++k) A4[k] = load_pack<float, 4, VEC>(a.A + at[k] + nc, left);
     const Pack<T, 4> B = load_pack<T, 4, false>(bp + nc, left), C = load_pack<T, 4, false>(cp + nc, left);
     if (n0 == 0) {
-      const float v = dt + bias;
+      const float v = to_f(dt) + bias;
       delta = a.softplus ? softplus(v) : v;
-      u = delta * x;
+      u = delta * to_f(x);
     }
     unsigned long long b[2], c[2];
 #pragma unroll
@@ -325,7 +322,7 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
       for (int q = 0; q < 2; ++q) {
         float e0, e1;
         unpack_f2(mul_f2(pack_f2(d2, d2), pack_f2(A4[k].v[2 * q], A4[k].v[2 * q + 1])), e0, e1);
-        const unsigned long long hs = fma_f2(pack_f2(ex2(e0), ex2(e1)), pack_f2(h[k].v[2 * q], h[k].v[2 * q + 1]), mul_f2(pack_f2(uk, uk), b[q]));
+        const unsigned long long hs = fma_f2(pack_f2(ex2(e0), ex2(e1)), pack_f2(from_slot >= 0 ? h[k].v[2 * q] : 0.f, from_slot >= 0 ? h[k].v[2 * q + 1] : 0.f), mul_f2(pack_f2(uk, uk), b[q]));
         unpack_f2(hs, h[k].v[2 * q], h[k].v[2 * q + 1]);
         unsigned long long hc = hs;   // (states past the end: the last one's again, which may be infinite, and no 0 x inf is added)
         if constexpr (!VEC) hc = pack_f2(2 * q < there ? h[k].v[2 * q] : 0.f, 2 * q + 1 < there ? h[k].v[2 * q + 1] : 0.f);
@@ -351,8 +348,8 @@ __global__ void __launch_bounds__(128, 6) ssm_step_kernel(const SsmArgs a, const
       y[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
   }
-  float out = a.D ? fmaf(skip, x, y[0]) : y[0];
-  if (a.z) out *= silu(z);
+  float out = a.D ? fmaf(skip, to_f(x), y[0]) : y[0];
+  if (a.z) out *= silu(to_f(z));
   if (lane < CPT && ch0 + lane < ch_end) reinterpret_cast<T *>(a.out)[row * a.ldo + ch0 + lane] = from_f<T>(out);
 }
 template <typename T, int L, bool VEC>
