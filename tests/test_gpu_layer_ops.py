@@ -728,3 +728,72 @@ def test_layer_captured_and_replayed(pkg):
             torch.cuda.synchronize()
             assert torch.equal(graphs[name][1], want), (i, name)
     assert torch.equal(layer.conv, eager.conv) and torch.equal(layer.ssm, eager.ssm)
+
+
+def test_offsets_past_32_bits(pkg):
+    """rows and slots so far apart that elements and bytes between the first and the last pass 2^31 and 2^32: what they give side by side"""
+    rows, d, n, far = 40, 64, 16, 2 ** 26 + 8
+    space = torch.empty(rows * far, dtype=BF16, device="cuda")             # 5.4 GB, of which a few rows are touched
+    assert (rows - 1) * far > 2 ** 31
+
+    def spread(t, at):
+        v = space.as_strided((rows, t.shape[1]), (far, 1), at)
+        v.copy_(t)
+        return v
+
+    x, dt, A, B, C, D, z, bias = _ssm_inputs(rows, d, n, 1, BF16)
+    fx, fdt, fB, fC, fz = (spread(t, at) for t, at in ((x, 0), (dt, 128), (B, 256), (C, 320), (z, 384)))
+    fout = spread(torch.zeros_like(x), 512)
+    w, b = _rand(96, d, dtype=BF16, scale=0.1, seed=3), _rand(d, 4, seed=4)
+    for m in (8, rows):
+        assert torch.equal(pkg.linear(fx[-m:], w), pkg.linear(x[-m:].contiguous(), w))
+        y = spread(torch.zeros((rows, 96), dtype=BF16, device="cuda"), 640)[-m:]
+        pkg.linear(fx[-m:], w, residual=y, out=y)
+        assert torch.equal(y, pkg.linear(x[-m:].contiguous(), w))
+    assert torch.equal(pkg.conv_seq(fx, b, out=fout), pkg.conv_seq(x, b))
+    assert torch.equal(pkg.conv_step(fx, b, out=fout), pkg.conv_step(x, b))
+    kw = dict(D=D, dt_bias=bias)
+    assert torch.equal(pkg.ssm_seq(fx, fdt, A, fB, fC, z=fz, out=fout, **kw), pkg.ssm_seq(x, dt, A, B, C, z=z, **kw))
+    assert torch.equal(pkg.ssm_step(fx, fdt, A, fB, fC, z=fz, out=fout, **kw), pkg.ssm_step(x, dt, A, B, C, z=z, **kw))
+    del space, fx, fdt, fB, fC, fz, fout, y
+    store = torch.empty(rows * far, dtype=F32, device="cuda")              # 10.7 GB
+    pool, near = store.as_strided((rows, d, n), (far, n, 1)), _rand(rows, d, n, seed=5)
+    pool.copy_(near)
+    order, first = list(range(rows - 1, -1, -1)), [rows - 1 - i for i in range(rows)]
+    pkg.copy_slots(pool, order, list(range(rows)))
+    pkg.copy_slots(near, order, list(range(rows)))
+    assert torch.equal(pool, near)
+    assert torch.equal(pkg.ssm_step(x, dt, A, B, C, state=pool, from_slots=first, to_slots=first, **kw),
+                       pkg.ssm_step(x, dt, A, B, C, state=near, from_slots=first, to_slots=first, **kw))
+    assert torch.equal(pool, near)
+    starts = [0, 7, 7, rows]
+    assert torch.equal(pkg.ssm_seq(x, dt, A, B, C, state=pool, starts=starts, from_slots=[39, 0, 38], to_slots=[39, 37, 38], **kw),
+                       pkg.ssm_seq(x, dt, A, B, C, state=near, starts=starts, from_slots=[39, 0, 38], to_slots=[39, 37, 38], **kw))
+    assert torch.equal(pool, near)
+
+
+def test_more_sequences_than_a_launch_holds(pkg):
+    lengths = [(i * 7) % 5 for i in range(600)]
+    starts = np.cumsum([0] + lengths).tolist()
+    rows, d, n = starts[-1], 24, 8
+    to = [(i * 77) % 601 for i in range(600)]
+    fro = [t if i % 3 else -1 for i, t in enumerate(to)]
+    x, w, b = _rand(rows, d, dtype=F16), _rand(d, 4, seed=1), _rand(d, seed=2)
+    pool = _rand(601, 3, d, dtype=F16, seed=3)
+    p = pool.clone()
+    want, err, new = _conv_want(x, w, b, "silu", starts, pool, fro, to)
+    _check(pkg.conv_seq(x, w, b, starts=starts, state=p, from_slots=fro, to_slots=to), want, err)
+    assert torch.equal(p, new)
+    x, dt, A, B, C, D, z, bias = _ssm_inputs(rows, d, n, 1, F16)
+    pool = _rand(601, d, n, seed=4)
+    p = pool.clone()
+    y, ey, new, enew = _ssm_want(x, dt, A, B, C, D, z, bias, True, starts, pool, fro, to)
+    _check(pkg.ssm_seq(x, dt, A, B, C, D=D, z=z, dt_bias=bias, starts=starts, state=p, from_slots=fro, to_slots=to), y, ey)
+    _check(p, new, enew)
+
+
+@pytest.mark.parametrize("k,n", [(72, 40), (71, 39), (8, 264)])
+def test_linear_of_many_rows(pkg, k, n):
+    x, w, b = _rand(100003, k, dtype=F16), _rand(n, k, dtype=F16, scale=0.2, seed=1), _rand(n, seed=2)
+    want, err = _linear_want(x, w, b, "silu", None)
+    _check(pkg.linear(x, w, b, activation="silu"), want, err)
