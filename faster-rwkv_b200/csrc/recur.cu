@@ -391,7 +391,7 @@ int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots) {
 }
 
 // Pieces of 2^shift rows, or 0: sequences whole.  Long sequences of few channels: their pieces side by side, twice the work, as long as that leaves a CTA
-// or two for every SM.  One of 4096 rows and 768 channels 79 us whole, 68 in pieces of 256 rows; of 256 channels 27 in pieces.
+// or two for every SM.  One of 4096 rows and 768 channels 80 us whole, 67 in pieces of 256 rows; of 256 channels 27 in pieces.
 int ssm_split(int64_t rows, int n_seq, int d) {
   const int64_t units = (int64_t)((d + 31) / 32) * n_seq;
   if (units > 24 || rows < 1024ll * n_seq) return 0;

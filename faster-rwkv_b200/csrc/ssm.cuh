@@ -40,6 +40,11 @@ template <typename T, int NS, int L>
 struct SsmTile {
   static constexpr int CH = SSM_STATES / L, NP = NS * L, YS = CH + 8;   // (YS: L rows of 32 / L channels in 32 banks)
   T in[SSM_RING][3][SSM_ROWS][CH + 16 / sizeof(T)];   // x, dt, z
+  // B and C as they lie, by the 16-byte words that a row touches (a word that holds one byte of it can be read), a tile ahead: loaded element by element they
+  // keep the helpers waiting (4096 rows of 4096 channels 171 us so).  More than 16 states: element by element (32: 142 us against 145 by words).
+  static constexpr bool WORDS = NP <= 16;
+  static constexpr int ROW_WORDS = WORDS ? (NP * (int)sizeof(T) + 30) / 16 : 1;
+  uint4 raw[WORDS ? 2 : 1][2][WORDS ? SSM_ROWS : 1][ROW_WORDS];
   float delta[2][CH][SSM_LD], u[2][CH][SSM_LD];      // time steps, times x
   float b[2][NP][SSM_LD], c[2][NP][SSM_LD];          // state n where bc_at says: the states that the lanes read at a time lie side by side
   static __device__ __forceinline__ int bc_at(int n) { return n % NS * L + n / NS; }
@@ -188,7 +193,8 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
     }
   const T *src[3] = {reinterpret_cast<const T *>(a.x) + ch0, reinterpret_cast<const T *>(a.dt) + ch0, reinterpret_cast<const T *>(a.z ? a.z : a.x) + ch0};
   const long long ld[3] = {a.ldx, a.lddt, a.z ? a.ldz : a.ldx};
-  // Rows and channels past the end repeat the last (and count for nothing): a load that is made or not is waited for where its ways meet.
+  // Rows and channels past the end count for nothing.  Copies leave the rows out; loads repeat the last: one that is made or not is waited for where
+  // its ways meet.
   constexpr int UNIT = 16 / (int)sizeof(T), ROW_UNITS = CH / UNIT, COPIES = SSM_ROWS * ROW_UNITS, PER = (COPIES + SSM_HELP - 1) / SSM_HELP;
   constexpr int SINGLE = SSM_ROWS * CH / SSM_HELP;
   T hold[VEC ? 1 : 3 * SINGLE];
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
           const int e = tid + q * SSM_HELP, r = e / ROW_UNITS, c = e % ROW_UNITS * UNIT;
-          if (e < COPIES) copy_async16(&sm.in[k % SSM_RING][arr][r][c], src[arr] + (t0 + min(r, final_row)) * ld[arr] + min(c, (ch_left - 1) / UNIT * UNIT));
+          if (e < COPIES && r <= final_row) copy_async16(&sm.in[k % SSM_RING][arr][r][c], src[arr] + (t0 + r) * ld[arr] + min(c, (ch_left - 1) / UNIT * UNIT));
         }
       } else {
 #pragma unroll
@@ -222,37 +228,55 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
     }
   };
   // B and C: four rows of a column at a time; columns past the last are 0
-  constexpr int FOURS = NP * (SSM_ROWS / 4), EACH4 = (FOURS + SSM_HELP - 1) / SSM_HELP, BATCH = EACH4 < 2 ? EACH4 : 2;
-  const T *bp = reinterpret_cast<const T *>(a.B) + (long long)group * a.n, *cp = reinterpret_cast<const T *>(a.C) + (long long)group * a.n;
-  struct { T b[4], c[4]; } bc[BATCH];
+  constexpr int FOURS = NP * (SSM_ROWS / 4), EACH4 = (FOURS + SSM_HELP - 1) / SSM_HELP, BATCH = Tile::WORDS ? 1 : EACH4 < 2 ? EACH4 : 2;
+  const T *bc_src[2] = {reinterpret_cast<const T *>(a.B) + (long long)group * a.n, reinterpret_cast<const T *>(a.C) + (long long)group * a.n};
+  const long long bc_ld[2] = {a.ldb, a.ldc};
+  constexpr int BC = MODE == SSM_ENDS ? 1 : 2;   // (no C)
+  auto words_ask = [&](int k) {   // tile k: its words on their way
+    const long long t0 = row + (long long)k * SSM_ROWS;
+    const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
+#pragma unroll
+    for (int m = 0; m < BC; ++m)
+#pragma unroll
+      for (int e = tid; e < SSM_ROWS * Tile::ROW_WORDS; e += SSM_HELP) {
+        const int r = e / Tile::ROW_WORDS, w = e % Tile::ROW_WORDS;
+        const uintptr_t p = reinterpret_cast<uintptr_t>(bc_src[m] + (t0 + r) * bc_ld[m]);
+        if (r <= final_row) copy_async16(&sm.raw[k & 1][m][r][w], reinterpret_cast<const uint4 *>(p & ~(uintptr_t)15) + min(w, (int)((p & 15) + a.n * sizeof(T) - 1) >> 4));
+      }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  T bc[BATCH][BC][4];
   auto bc_ask = [&](int k, int q0) {
     const long long t0 = row + (long long)k * SSM_ROWS;
     const int final_row = (int)min(end - 1 - t0, (long long)SSM_ROWS - 1);
-    const T *b = bp + t0 * a.ldb, *c = cp + t0 * a.ldc;
+    const T *base[2] = {bc_src[0] + t0 * a.ldb, bc_src[1] + t0 * a.ldc};
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
       const int e = tid + (q0 + q) * SSM_HELP, col = min(e % NP, a.n - 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = min(e / NP * 4 + i, final_row);
-        bc[q].b[i] = b[r * a.ldb + col];
-        if (MODE != SSM_ENDS) bc[q].c[i] = c[r * a.ldc + col];
-      }
+      for (int m = 0; m < BC; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = e / NP * 4 + i;
+          if constexpr (Tile::WORDS) {
+            const uint32_t off = ((uint32_t)reinterpret_cast<uintptr_t>(base[m]) + (uint32_t)r * (uint32_t)bc_ld[m] * (uint32_t)sizeof(T)) & 15;
+            bc[q][m][i] = *reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(&sm.raw[k & 1][m][r % SSM_ROWS][0]) + off + col * sizeof(T));
+          } else {
+            bc[q][m][i] = base[m][min(r, final_row) * bc_ld[m] + col];
+          }
+        }
     }
   };
   auto bc_put = [&](int buf, int q0) {
 #pragma unroll
     for (int q = 0; q < BATCH; ++q) {
       const int e = tid + (q0 + q) * SSM_HELP, col = e % NP;
-      if (e < FOURS) {
-        float4 b, c;
-        b.x = to_f(bc[q].b[0]); b.y = to_f(bc[q].b[1]); b.z = to_f(bc[q].b[2]); b.w = to_f(bc[q].b[3]);
-        *reinterpret_cast<float4 *>(&sm.b[buf][Tile::bc_at(col)][e / NP * 4]) = col < a.n ? b : float4{};
-        if (MODE != SSM_ENDS) {
-          c.x = to_f(bc[q].c[0]); c.y = to_f(bc[q].c[1]); c.z = to_f(bc[q].c[2]); c.w = to_f(bc[q].c[3]);
-          *reinterpret_cast<float4 *>(&sm.c[buf][Tile::bc_at(col)][e / NP * 4]) = col < a.n ? c : float4{};
+      if (e < FOURS)
+#pragma unroll
+        for (int m = 0; m < BC; ++m) {
+          const float4 v = make_float4(to_f(bc[q][m][0]), to_f(bc[q][m][1]), to_f(bc[q][m][2]), to_f(bc[q][m][3]));
+          *reinterpret_cast<float4 *>(m ? &sm.c[buf][Tile::bc_at(col)][e / NP * 4] : &sm.b[buf][Tile::bc_at(col)][e / NP * 4]) = col < a.n ? v : float4{};
         }
-      }
     }
   };
   // rows out: two channels of every STRIDE-th row
@@ -263,16 +287,21 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
   for (int i = 0; i < 2; ++i) skip[i] = a.D && out_ch + i < ch_left ? a.D[ch0 + out_ch + i] : 0.f;
   T *op = reinterpret_cast<T *>(a.out) + ch0 + out_ch;
   if (tiles > 0) {
-    ask(0);
-    if (VEC) ask(1);   // (past the end too: the last row again)
-    bc_ask(0, 0);
+    if constexpr (VEC) ask(0);
+    if constexpr (Tile::WORDS) words_ask(0);
+    else bc_ask(0, 0);
+    ask(VEC ? 1 : 0);   // (past the end too: the last row again)
   }
   for (int k = 0; k <= tiles; ++k) {
     const int buf = k & 1;
     if (k < tiles) {
-      if (VEC) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else keep(k);
+      if constexpr (VEC) asm volatile("cp.async.wait_group 1;" ::: "memory");   // (all but the rows of tile k + 1)
+      else {
+        if (Tile::WORDS) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        keep(k);
+      }
       pair_sync<SSM_BAR_HELP, SSM_HELP>(0);   // everybody's part of tile k is there, and nobody is at tile k - 2 any more
+      if constexpr (Tile::WORDS) words_ask(k + 1);
       ask(k + (VEC ? 2 : 1));
       const long long t0 = row + (long long)k * SSM_ROWS;
       Pack<T, 2> x[BLOCKS], dt[BLOCKS];   // (all of them ahead of the first store, which a load would have to stay behind)
@@ -291,9 +320,14 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
           sm.delta[buf][g * 8 + in_ch + e][in_row] = v;
           sm.u[buf][g * 8 + in_ch + e][in_row] = v * to_f(x[g].v[e]);
         }
-      bc_put(buf, 0);
-      for (int q0 = BATCH; q0 < EACH4; q0 += BATCH) { bc_ask(k, q0); bc_put(buf, q0); }
-      bc_ask(k + 1, 0);
+      if constexpr (Tile::WORDS) {
+#pragma unroll
+        for (int q0 = 0; q0 < EACH4; q0 += BATCH) { bc_ask(k, q0); bc_put(buf, q0); }
+      } else {
+        bc_put(buf, 0);
+        for (int q0 = BATCH; q0 < EACH4; q0 += BATCH) { bc_ask(k, q0); bc_put(buf, q0); }
+        bc_ask(k + 1, 0);
+      }
       pair_arrive<SSM_BAR_FULL, SSM_THREADS>(buf);
     }
     if (k == 0) continue;
@@ -324,7 +358,7 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
       }
     }
   }
-  if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if constexpr (MODE == SSM_ENDS) {
     // the sum of a channel's time steps, over the rows' threads in a fixed order
 #pragma unroll
@@ -387,17 +421,17 @@ cudaError_t ssm_seq_split(const SsmArgs &a, const SeqTable &t, cudaStream_t st) 
   if (e == cudaSuccess) e = op_launch(ssm_join_kernel, dim3((unsigned)(((size_t)a.d * a.n + 255) / 256), t.n), 256, 0, st, 1, a, t);
   return e == cudaSuccess ? ssm_seq_mode<T, NS, L, 2, SSM_PIECE, VEC>(a, t, items, st) : e;
 }
-// States a lane.  Few channels and sequences: fewer states, more CTAs and the shorter chain (4096 rows of 768 channels with 16 states: 79 us with one a
-// lane, 106 with two, 183 with four; of 1536: 121, 106, 183; of 4096: 251, 171, 186; two sequences of 4096: 251, 170, 145; 1000 rows of
-// 2048 with 64: 84 with four a lane, 93 with eight; 4096 of 4096 with 8: 149 with one, 163 with two).  Many: three CTAs an SM where
-// their registers allow it (11 sequences of 5120 channels 117 us against 128; one of 4096 190 against 186).
+// States a lane.  Few channels and sequences: fewer states, more CTAs and the shorter chain (4096 rows of 768 channels with 16 states: 80 us with one a
+// lane, 107 with two, 185 with four; of 1536: 119, 107, 185; of 4096: 235, 167, 187; two sequences of 4096: 215, 167, 144; 1000 rows of
+// 2048 with 64: 84 with four a lane, 89 with eight; 4096 of 2048 with 8: 105 with one, 141 with two; of 4096: 144, 142).  Many: three
+// CTAs an SM where their registers allow it (11 sequences of 5120 channels 117 us against 127; one of 4096 198 against 187).
 template <typename T, bool VEC>
 cudaError_t ssm_seq_any(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {
   auto ctas = [&](int ch) { return (long long)((a.d / a.groups + ch - 1) / ch) * a.groups * t.n; };
   const int sms = device_sm_count();
   if (a.n <= 8) {
     if (a.shift) return ssm_seq_split<T, 2, 4, VEC>(a, t, st);
-    if (ctas(16) <= 2 * sms) return ssm_seq_mode<T, 1, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
+    if (ctas(16) <= sms) return ssm_seq_mode<T, 1, 8, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     if (ctas(32) <= 2 * sms) return ssm_seq_mode<T, 2, 4, 2, SSM_WHOLE, VEC>(a, t, t.n, st);
     return ssm_seq_mode<T, 2, 4, 3, SSM_WHOLE, VEC>(a, t, t.n, st);
   }
