@@ -94,6 +94,8 @@ SIGNATURES = {
     "fr_b200_matmul": (_i, [_vp, _i, _i, _i, _vp, _i, _i, _vp, _i, _i, _vp]),
     "fr_b200_linear_workspace": (_sz, [_vp, _i64, _vp, _i64, _i64, _i, _i]),
     "fr_b200_linear": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i, _i, _vp, _i, _vp, _i64, _vp, _i64, _i, _vp, _sz, _i, _vp]),
+    "fr_b200_op_status": (_i, [_i]),
+    "fr_b200_op_wait_selftest": (_i, [_i, ctypes.c_uint, _vp]),
     "fr_b200_conv_seq": (_i, [_vp, _i64, _i, _i64, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
     "fr_b200_conv_step": (_i, [_vp, _i64, _i, _i, _i, _vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i, _vp]),
     "fr_b200_ssm_seq_workspace": (_sz, [_i64, _i, _i, _i]),
@@ -437,4 +439,4 @@ def matvec(W: np.ndarray, x: np.ndarray, weight_format: int, device: int = 0) ->
 
 
 # operators of a recurrent layer over torch CUDA tensors
-from .ops import conv_seq, conv_step, copy_slots, linear, ssm_seq, ssm_step  # noqa: E402,F401
+from .ops import check_operators, conv_seq, conv_step, copy_slots, linear, ssm_seq, ssm_step  # noqa: E402,F401

@@ -270,8 +270,10 @@ __global__ void __launch_bounds__(32 * NW, CTAS) linear_rows_kernel(const Linear
 constexpr int LK = 64, L_THREADS = 192, ST_LINEAR_TIMEOUT = 301;
 constexpr uint32_t L_TILE = 128 * LK * 2;   // 128 rows of 64 inputs
 
-// a wait that gave up (a fault of the device; the output is not written): read by the next call
-__managed__ int linear_status;
+// The first wait of each device that gave up: what fr_b200_op_status() takes.
+constexpr int STATUS_DEVICES = 64;
+__managed__ int linear_status[STATUS_DEVICES];
+int *status_word(int device) { return &linear_status[std::min(std::max(device, 0), STATUS_DEVICES - 1)]; }
 
 // R rows of V channels each: the residuals are asked for ahead of the sums; bias, one branch for the activation, residual, one rounding
 template <typename T, bool OUT32, bool RES, int R, int V>
@@ -316,12 +318,20 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
                : "memory");
 }
 
+// Behind a wait that gave up: copies and MMAs that were asked for just before end while the CTA still has its shared and tensor memory
+// (they take microseconds; those of a place that the wait was for had two seconds).
+__device__ __forceinline__ void settle() {
+  const unsigned long long t0 = globaltimer_ns();
+  for (int i = 0; i < 10000 && globaltimer_ns() - t0 < 1000000ull; ++i) __nanosleep(1000);
+}
+
 struct LinearMaps { CUtensorMap x, w; };
 struct LinearPlan {
   int bn;            // MMA columns: rows of x (tile kernel), channels (pair kernel)
   int stages, split;
   int m_tiles, n_tiles;
   int vec;           // out and residual rows can be taken four elements at a time (tile kernel) / eight (pair kernel)
+  int *status;       // the device's word for waits that gave up
 };
 template <typename T>
 __host__ __device__ constexpr uint32_t linear_idesc(int m, int n) {   // kind::f16, D fp32; A and B fp16 (0) or bf16 (1) in bits 7-9 and 10-12
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
   if (warp == 0) {
     Ring at;
     for (int e = 0; e < nk; ++e, at.next(p.stages)) {
-      if (e >= p.stages && !__all_sync(0xffffffffu, mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, &linear_status, ST_LINEAR_TIMEOUT))) break;
+      if (e >= p.stages && !__all_sync(0xffffffffu, mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, p.status, ST_LINEAR_TIMEOUT))) break;
       if (elect_one()) {
         const uint32_t dst = tiles + (uint32_t)at.slot * stage;
         mbar_expect_tx(&full[at.slot], stage);
@@ -384,7 +394,7 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
     Ring at;
     bool ok = true;
     for (int e = 0; e < nk; ++e, at.next(p.stages)) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[at.slot], at.phase, abort_flag, &linear_status, ST_LINEAR_TIMEOUT))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[at.slot], at.phase, abort_flag, p.status, ST_LINEAR_TIMEOUT))) { ok = false; break; }
       tc_fence_after();
       const uint32_t base = tiles + (uint32_t)at.slot * stage;
       const uint64_t wd = umma_desc_k128(base), xd = umma_desc_k128(base + L_TILE);
@@ -399,7 +409,7 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
     __syncwarp();
   }
   // everybody waits for the sums: the ring is free then, and takes them as [row][128 channels]
-  const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag, &linear_status, ST_LINEAR_TIMEOUT));
+  const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag, p.status, ST_LINEAR_TIMEOUT));
   tc_fence_after();
   const int rows = min(p.bn, a.M - m0);
   if (ok && warp >= 2) {
@@ -412,7 +422,13 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(!ok)) {
+    // A wait gave up: NaN is what this CTA adds to its own rows and to those that others of its cluster finish.
+    settle();
+    if (warp >= 2)
+      for (int c = 0; c < rows; ++c) sts_u32(tiles + ((uint32_t)c * 128 + (warp & 3) * 32 + lane) * 4, 0x7fc00000u);
+    __syncthreads();
+  }
   // The tensor memory goes back before the CTA waits for the others of its cluster: held until they are done, it could be what one of them waits for,
   // by way of a third kernel's CTAs that hold the rest.
   if (warp == 1) {
@@ -422,7 +438,7 @@ __global__ void __launch_bounds__(L_THREADS) linear_tile_kernel(const LinearArgs
   if (p.split > 1) cluster_sync();
   // a warp finishes a row: four channels a lane.  Rows of the cluster's CTAs in turn.
   const int n = ch0 + lane * 4;
-  if (ok && n < a.N) {
+  if (n < a.N) {
     float bias[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) bias[i] = a.bias && n + i < a.N ? a.bias[n + i] : 0.f;
@@ -521,7 +537,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
       place(t, mt, nt);
       const int m0 = mt * 256 + (int)rank * 128, n0 = nt * p.bn + (int)rank * (p.bn / 2);
       for (int e = 0; e < num_k; ++e, at.next(LP_STAGES)) {
-        if (filled >= LP_STAGES && !__all_sync(0xffffffffu, mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, &linear_status, ST_LINEAR_TIMEOUT))) { ok = false; break; }
+        if (filled >= LP_STAGES && !__all_sync(0xffffffffu, mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, p.status, ST_LINEAR_TIMEOUT))) { ok = false; break; }
         if (filled < LP_STAGES) ++filled;
         if (elect_one()) {
           const uint32_t dst = tiles + (uint32_t)at.slot * LP_STAGE, bar = mapa_u32(smem_u32(&full[at.slot]), 0);
@@ -540,10 +556,10 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += pairs, ++i) {
         const int buf = i & 1;
-        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], (uint32_t)((i >> 1) - 1) & 1u, abort_flag, &linear_status, ST_LINEAR_TIMEOUT))) break;
+        if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&acc_empty[buf], (uint32_t)((i >> 1) - 1) & 1u, abort_flag, p.status, ST_LINEAR_TIMEOUT))) break;
         tc_fence_after();
         for (int e = 0; e < num_k; ++e, at.next(LP_STAGES)) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&full[at.slot], at.phase, abort_flag, &linear_status, ST_LINEAR_TIMEOUT))) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, mbar_wait(&full[at.slot], at.phase, abort_flag, p.status, ST_LINEAR_TIMEOUT))) { ok = false; break; }
           tc_fence_after();
           const uint32_t base = tiles + (uint32_t)at.slot * LP_STAGE;
           const uint64_t xd = umma_desc_k128(base), wd = umma_desc_k128(base + L_TILE);
@@ -563,11 +579,18 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
     const int quad = warp & 3, half = (warp - 2) >> 2, sub = lane & 3;
     const uint32_t out_at = tiles + LP_STAGES * LP_STAGE + (uint32_t)(warp - 2) * LP_OUT, bias_at = tiles + LP_STAGES * LP_STAGE + 8 * LP_OUT + (uint32_t)(warp - 2) * 128;
     int i = 0;
+    bool good = true;
     for (int t = pair; t < num_tiles; t += pairs, ++i) {
       int mt, nt;
       place(t, mt, nt);
       const int buf = i & 1, m0 = mt * 256 + (int)rank * 128 + quad * 32, n0 = nt * p.bn;
-      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (uint32_t)(i >> 1) & 1u, abort_flag, &linear_status, ST_LINEAR_TIMEOUT))) break;
+      good = good && __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (uint32_t)(i >> 1) & 1u, abort_flag, p.status, ST_LINEAR_TIMEOUT));
+      if (!good) {   // a wait gave up: NaN in this tile and those behind it
+        using O = typename std::conditional<OUT32, float, T>::type;
+        for (int ch = n0 + 32 * half + lane; ch < min(n0 + p.bn, a.N); ch += 64)
+          for (int r = 0; r < 32 && m0 + r < a.M; ++r) reinterpret_cast<O *>(a.out)[(long long)(m0 + r) * a.ldo + ch] = from_f<O>(__uint_as_float(0x7fc00000u));
+        continue;
+      }
       tc_fence_after();
       const uint32_t tm = tmem + (uint32_t)buf * 256 + ((uint32_t)(quad * 32) << 16);
       uint32_t acc[32];
@@ -657,7 +680,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (__syncthreads_or(*abort_flag)) settle();
   cluster_sync();   // neither CTA leaves while the other's MMAs, commits or arrivals may reach into it
   if (warp == 1) {
     tc_fence_after();
@@ -687,7 +710,7 @@ cudaError_t rows_launch(const LinearArgs &a, cudaStream_t st) {
   return a.M <= 8 ? rows_any<T, 1, 4, 2, VEC>(a, st) : a.M <= 16 ? rows_any<T, 2, 4, 2, VEC>(a, st) : rows_any<T, 4, 3, 1, VEC>(a, st);
 }
 template <typename T>
-cudaError_t tile_launch(const LinearArgs &a, int bn, int split, cudaStream_t st) {
+cudaError_t tile_launch(const LinearArgs &a, int bn, int split, int *status, cudaStream_t st) {
   static thread_local uint64_t told[4];
   const int kind = a.out_f32 * 2 + (a.residual != nullptr);
   const auto kern = kind == 0 ? linear_tile_kernel<T, false, false> : kind == 1 ? linear_tile_kernel<T, false, true>
@@ -696,7 +719,7 @@ cudaError_t tile_launch(const LinearArgs &a, int bn, int split, cudaStream_t st)
   if (e != cudaSuccess) return e;
   LinearPlan p;
   LinearMaps maps;
-  p.bn = bn;
+  p.bn = bn; p.status = status;
   p.n_tiles = (a.N + 127) / 128; p.m_tiles = (a.M + bn - 1) / bn;
   const uint32_t stage = L_TILE + (uint32_t)bn * LK * 2;
   split = std::min(split, (a.K + LK - 1) / LK);
@@ -711,7 +734,7 @@ cudaError_t tile_launch(const LinearArgs &a, int bn, int split, cudaStream_t st)
   return op_launch(kern, dim3(p.n_tiles * split, p.m_tiles), L_THREADS, 2048 + (size_t)p.stages * stage, st, split, a, p, maps);
 }
 template <typename T>
-cudaError_t pair_launch(const LinearArgs &a, int bn, cudaStream_t st) {
+cudaError_t pair_launch(const LinearArgs &a, int bn, int *status, cudaStream_t st) {
   static thread_local uint64_t told[4];
   const int kind = a.out_f32 * 2 + (a.residual != nullptr);
   const auto kern = kind == 0 ? linear_pair_kernel<T, false, false> : kind == 1 ? linear_pair_kernel<T, false, true>
@@ -720,7 +743,7 @@ cudaError_t pair_launch(const LinearArgs &a, int bn, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   LinearPlan p;
   LinearMaps maps;
-  p.bn = bn; p.split = 1; p.stages = LP_STAGES;
+  p.bn = bn; p.split = 1; p.stages = LP_STAGES; p.status = status;
   p.m_tiles = (a.M + 255) / 256; p.n_tiles = (a.N + bn - 1) / bn;
   p.vec = a.ldo % 8 == 0 && aligned(a.out, a.out_f32 ? 32 : 16) && (!a.residual || (a.ldr % 8 == 0 && aligned(a.residual, a.out_f32 ? 32 : 16)));
   if (!rows_map(&maps.x, a.x, a.M, a.K, a.ldx, 128) || !rows_map(&maps.w, a.w, a.N, a.K, a.ldw, bn / 2)) return cudaErrorInvalidValue;
@@ -814,7 +837,7 @@ cudaError_t any_launch(const LinearArgs &a, cudaStream_t st) {
   return op_launch(linear_any_kernel<T>, dim3(nt * split, mt), 128, 0, st, split, a, split);
 }
 template <typename T>
-cudaError_t linear_launch(LinearArgs a, uint8_t *work, cudaStream_t st) {
+cudaError_t linear_launch(LinearArgs a, uint8_t *work, int *status, cudaStream_t st) {
   if (work) {
     cudaError_t e = align_launch(&a.x, &a.ldx, a.M, a.K, &work, st);
     if (e == cudaSuccess) e = align_launch(&a.w, &a.ldw, a.N, a.K, &work, st);
@@ -823,7 +846,7 @@ cudaError_t linear_launch(LinearArgs a, uint8_t *work, cudaStream_t st) {
   if (!whole_rows(a.x, a.ldx) || !whole_rows(a.w, a.ldw)) return a.M <= 32 ? rows_launch<T, false>(a, st) : any_launch<T>(a, st);
   const LinearChoice c = linear_choice(a.M, a.K, a.N);
   if (c.rows) return rows_launch<T, true>(a, st);
-  return c.pair ? pair_launch<T>(a, c.bn, st) : tile_launch<T>(a, c.bn, c.split, st);
+  return c.pair ? pair_launch<T>(a, c.bn, status, st) : tile_launch<T>(a, c.bn, c.split, status, st);
 }
 
 }  // namespace
@@ -860,12 +883,29 @@ int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int d
   OP_CU(dev.enter(device));
   LinearArgs a{x, w, residual, bias, out, ldx, ldw, ldr, ldo, (int)rows, N, K, act, out_dtype == FR_B200_T_F32};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (linear_status) {
-    linear_status = 0;
-    return op_fail(FR_B200_E_TIMEOUT, "a wait of an earlier linear call gave up; its result is not there");
-  }
-  if (dtype == FR_B200_T_F16) OP_CU(linear_launch<__half>(a, need ? reinterpret_cast<uint8_t *>(work) : nullptr, st));
-  else OP_CU(linear_launch<__nv_bfloat16>(a, need ? reinterpret_cast<uint8_t *>(work) : nullptr, st));
+  if (dtype == FR_B200_T_F16) OP_CU(linear_launch<__half>(a, need ? reinterpret_cast<uint8_t *>(work) : nullptr, status_word(device), st));
+  else OP_CU(linear_launch<__nv_bfloat16>(a, need ? reinterpret_cast<uint8_t *>(work) : nullptr, status_word(device), st));
+  return FR_B200_OK;
+  OP_CATCH
+}
+
+// (the word is read and cleared in one step: no wait that gives up in between is lost)
+int fr_b200_op_status(int device) {
+  OP_TRY
+  DeviceScope dev;
+  OP_CU(dev.enter(device));
+  const int code = __atomic_exchange_n(status_word(device), 0, __ATOMIC_ACQ_REL);
+  if (code) return op_fail(FR_B200_E_TIMEOUT, "a device-side wait of an operator gave up (code " + std::to_string(code) + "): NaN stands in its result");
+  return FR_B200_OK;
+  OP_CATCH
+}
+
+int fr_b200_op_wait_selftest(int device, unsigned limit_us, void *stream) {
+  OP_TRY
+  OP_REQUIRE(limit_us >= 1 && limit_us <= 1000000, "limit must be 1 .. 1,000,000 microseconds");
+  DeviceScope dev;
+  OP_CU(dev.enter(device));
+  OP_CU(launch_wait_selftest(status_word(device), (unsigned long long)limit_us * 1000ull, reinterpret_cast<cudaStream_t>(stream)));
   return FR_B200_OK;
   OP_CATCH
 }

@@ -55,6 +55,13 @@ def linear(x, w, bias=None, activation="none", residual=None, out=None, out_dtyp
     return _done((_ext or _load()).linear(x, w, bias, _act(activation), residual, out, out_dtype), "fr_b200_linear")
 
 
+def check_operators(device=0):
+    """Raises if a device-side wait of an operator gave up on `device` since the last check (NaN stands in the result of that call then).  It does
+    not synchronise: torch.cuda.synchronize() comes before it."""
+    from . import lib
+    _done(lib().fr_b200_op_status(int(device)) or None, "fr_b200_op_status")
+
+
 def conv_seq(x, w, bias=None, activation="silu", starts=None, state=None, from_slots=None, to_slots=None, out=None):
     """Causal convolution of each channel over the last taps rows of its sequence: x [rows, D], w [D, taps] (2 to 4) and bias
     [D] fp32, activation none or silu.  starts: first rows of the sequences and the end of the last (None: one sequence).

@@ -279,6 +279,8 @@ const char *fr_b200_op_last_error(void);
  *   - asynchronous on `stream`, on `device` whatever device is current (the caller's stays current); nothing is allocated,
  *     nothing is synchronised, no result depends on the order of atomics: calls may be captured, and captured calls hold
  *     the host arrays (sequences, slots) by value;
+ *   - waits inside fr_b200_linear's kernels are bounded.  Where one gives up (a fault of the device) the rows concerned hold NaN, also
+ *     when a captured call is replayed, no other call is refused, and fr_b200_op_status() tells;
  *   - host arrays are checked: FR_B200_E_ARG, with the reason in fr_b200_op_last_error(), and nothing is launched.
  *     Outputs may not overlap inputs or the pool, except where it says so;
  *   - sequences: `starts` (host [n_seq + 1], not decreasing, within 0 .. rows) gives sequence i the rows starts[i] ..
@@ -296,6 +298,12 @@ const char *fr_b200_op_last_error(void);
 size_t fr_b200_linear_workspace(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t rows, int K, int N);
 int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int dtype, int64_t rows, int K, int N, const float *bias, int act,
                    const void *residual, int64_t ldr, void *out, int64_t ldo, int out_dtype, void *work, size_t work_bytes, int device, void *stream);
+
+/* FR_B200_E_TIMEOUT if a wait of an operator gave up on this device since the call before, else 0.  It does not wait for the device:
+ * work that is to be judged has been synchronised with before. */
+int fr_b200_op_status(int device);
+/* fr_b200_wait_selftest for the operators: a wait of limit_us microseconds that runs out, on `stream`; fr_b200_op_status() tells of it then. */
+int fr_b200_op_wait_selftest(int device, unsigned limit_us, void *stream);
 
 /* y[t, d] = act(bias[d] + sum_j w[d, j] x[t - (taps - 1) + j, d]), act none or silu, taps 2 to 4; w [D, taps], bias [D] or NULL.
  * A state is the last taps - 1 rows, [taps - 1, D] in the type of x, oldest first: they come before a sequence's first row. */
