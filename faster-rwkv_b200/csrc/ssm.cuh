@@ -374,6 +374,17 @@ __global__ void __launch_bounds__(SSM_THREADS, CTAS) ssm_seq_kernel(const SsmArg
   }
 }
 
+// What S becomes along a piece: 2^arg S + end, arg = log2 e A times the sum of the piece's time steps.  Row by row a state passes through decays that
+// are all in range, though their product may not be: beyond 2^+-120 it is taken in three factors, between which no value leaves the range that
+// S and the result have.  From 0 a state comes as from zero (not 0 x inf), and an infinite one stays infinite
+// (not inf x 0) unless the decay of a row is 0 itself: A or a time step is infinite.
+__device__ __forceinline__ float ssm_carry(float S, float arg, float end) {
+  if (fabsf(arg) <= 120.f) return fmaf(ex2(arg), S, end);
+  const float t = ex2(arg * (1.f / 3.f));
+  if (S == 0.f || (t == 0.f && isinf(S) && !isinf(arg))) return S + end;
+  return fmaf(S * t * t, t, end);
+}
+
 // The pieces' states from zero -> the states that they begin with, in their place: S <- exp(A sum of time steps) S + end.
 // One thread per channel and state of a sequence.
 static __global__ void __launch_bounds__(256) ssm_join_kernel(const SsmArgs a, const __grid_constant__ SeqTable tab) {
@@ -400,7 +411,7 @@ static __global__ void __launch_bounds__(256) ssm_join_kernel(const SsmArgs a, c
     for (int i = 0; i < AHEAD; ++i) {
       if (p0 + i >= pieces) break;
       w[(size_t)(p0 + i) * (dn + a.d) + e] = S;
-      S = fmaf(ex2(sum[i] * A2), S, end[i]);
+      S = ssm_carry(S, sum[i] * A2, end[i]);
     }
   }
 }

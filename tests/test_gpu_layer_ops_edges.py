@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_layer_ops import F16, F32, _check, _linear_want, _rand
+from test_gpu_layer_ops import BF16, EX2, F16, F32, U32, _check, _linear_want, _rand, _ssm_inputs, _ssm_want
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,60 @@ def test_a_wait_that_gave_up_is_told_once_and_refuses_nobody(pkg):
     with pytest.raises(pkg.FrB200Error):
         pkg.check_operators(0)
     pkg.check_operators(0)
+
+
+# ---- long narrow prompts: pieces of a sequence side by side ------------------------------------------------------
+
+def _cut(pkg, rows, d, n):
+    assert pkg.lib().fr_b200_ssm_seq_workspace(rows, 1, d, n) > 0
+
+
+@pytest.mark.parametrize("d,n,dtype,bias", [(24, 5, F16, -1.0), (13, 16, F32, -3.0), (10, 3, BF16, -1.0), (8, 70, F32, -4.0)])
+def test_ssm_pieces_with_infinite_inputs(pkg, d, n, dtype, bias):
+    """an infinite x, or an infinite state to begin with, makes its channel infinite to the end, however far the decay of a whole piece falls (that
+    of a row stays in the range of fp32)"""
+    rows = 1100
+    _cut(pkg, rows, d, n)
+    x, dt, A, B, C, D, z, _ = _ssm_inputs(rows, d, n, 1, dtype)
+    bias = torch.full((d,), bias, device="cuda")
+    step = torch.nn.functional.softplus(dt.double() + bias)
+    assert float(step.max() * -A.min()) < 80 and float(step[:256].sum(0).max() * -A.min()) > 100
+    x, B, C = x.clone(), B.abs().contiguous(), C.abs().contiguous()
+    B[B == 0], C[C == 0] = 0.5, 0.5
+    x[7, 4], x[300, 6] = float("inf"), float("-inf")
+    start = torch.zeros((2, d, n), device="cuda")
+    start[0, 5] = float("inf")
+    y, ey, new, enew = _ssm_want(x, dt, A, B, C, None, z, bias, True, [0, rows], start, [0], [1])
+    for c, t in ((4, 7), (5, 0), (6, 300)):
+        assert torch.isinf(y[t:, c]).all()
+    p = start.clone()
+    got = pkg.ssm_seq(x, dt, A, B, C, z=z, dt_bias=bias, state=p, from_slots=[0], to_slots=[1])
+    # a piece's decay is the exponential of a sum of up to 256 time steps, off by as many roundings of it: |x| exp(-|x|) <= 0.37 of the state
+    extra = 256 * U32 * 0.37 * max(1.0, float(new[torch.isfinite(new)].abs().max()))
+    _check(got, y, ey + extra * C.double().abs().sum(1, keepdim=True) * (z.double().abs() + 1), "out")
+    _check(p, new, enew + extra, "state")
+
+
+def test_ssm_pieces_whose_decays_leave_the_range(pkg):
+    """products of a piece's decays beyond the range of fp32, where no row's are: states that are 0 stay so while decays grow, small ones grow
+    to ordinary ones, large ones fall to
+    them.  The decay of a piece is 2^arg with arg off by 44 roundings (a sum of 256 time steps in
+    partial sums of 8 and 32, times A, log2 e and a third), cubed: 44 U32 |arg| + 3 EX2 + 4 U32 of the value."""
+    rows, d, n = 1100, 4, 3
+    _cut(pkg, rows, d, n)
+    x, dt = torch.zeros((rows, d), device="cuda"), torch.zeros((rows, d), device="cuda")
+    B, C = _rand(rows, n).abs() + 0.1, _rand(rows, n, seed=1).abs() + 0.1
+    A = torch.tensor([0.5, 0.35, -0.4, -0.39], device="cuda")[:, None] * torch.ones(n, device="cuda")
+    x[1050:, 0] = _rand(50, seed=2).abs()
+    dt[:, 0] = 1.0                     # from zero: grows by 2^184 a piece, with nothing to grow before row 1050
+    dt[:256, 1:] = 1.0                 # 1e-30 by 2^129, 1e30 by 2^-148, 1e36 by 2^-144; then unchanged
+    x[1050:, 1:] = 1e-3
+    start = torch.zeros((1, d, n), device="cuda")
+    start[0, 1], start[0, 2], start[0, 3] = 1e-30, 1e30, 1e36
+    y, ey, new, enew = _ssm_want(x, dt, A, B, C, None, None, None, False, [0, rows], start, [0], [0])
+    assert torch.isfinite(y).all() and float(new[0, 1].min()) > 1e8 and 0 < float(new[0, 2].max()) < 1e-9
+    extra = 44 * U32 * 150 + 3 * EX2 + 4 * U32
+    p = start.clone()
+    got = pkg.ssm_seq(x, dt, A, B, C, dt_softplus=False, state=p)
+    _check(got, y, ey + extra * y.abs(), "out")
+    _check(p, new, enew + extra * new.abs(), "state")
