@@ -36,12 +36,30 @@ struct LinearArgs {
   int M, N, K, act, out_f32;
 };
 
+// v times the normal distribution's integral up to v.  Its tail Q(a) = exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.3 a), a = |v|: P fitted by least squares,
+// reweighted towards the largest error, to erfc's scaled form on 0 <= a <= 13.3; relative error 1.2e-7, some (8 + 0.7 v^2) 2^-24 with the roundings.
+// (1 + erf(v / sqrt 2) has lost the tail of v < 0: off by a tenth at -5, 0 from -5.7 on; erfcf() keeps it, but 4096 rows of
+// 64 x 5120 took 62 us with it, 35 so.)
+__device__ __forceinline__ float gelu(float v) {
+  const float a = fabsf(v), t = __fdividef(1.f, fmaf(a, 0.3f, 1.f));
+  float q = 0.0360364548f;
+  q = fmaf(q, t, -0.158714195f);
+  q = fmaf(q, t, 0.208965507f);
+  q = fmaf(q, t, -0.0560966438f);
+  q = fmaf(q, t, 0.129843779f);
+  q = fmaf(q, t, 0.0995229662f);
+  q = fmaf(q, t, 0.120816906f);
+  q = fmaf(q, t, 0.119625165f);
+  q *= t * ex2(a * a * (-0.5f * LOG2E));
+  return v * (v > 0.f ? 1.f - q : q);
+}
+
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
     case FR_B200_ACT_RELU2: return v < 0.f ? 0.f : v * v;   // (NaN stays NaN)
     case FR_B200_ACT_SILU: return silu(v);
     case FR_B200_ACT_SIGMOID: return __fdividef(1.f, 1.f + ex2(-v * LOG2E));
-    case FR_B200_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678f));
+    case FR_B200_ACT_GELU: return gelu(v);
     case FR_B200_ACT_SOFTPLUS: return softplus(v);
     default: return v;
   }

@@ -99,3 +99,19 @@ def test_ssm_pieces_whose_decays_leave_the_range(pkg):
     got = pkg.ssm_seq(x, dt, A, B, C, dt_softplus=False, state=p)
     _check(got, y, ey + extra * y.abs(), "out")
     _check(p, new, enew + extra * new.abs(), "state")
+
+
+# ---- activations -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [3, 60, 300])
+@pytest.mark.parametrize("out_dtype", [F16, F32])
+def test_gelu_keeps_its_negative_tail(pkg, rows, out_dtype):
+    """Values from the bias alone, exact in fp32: what the function itself is off by is relative, down to the smallest.  In half steps of fp32: the fit
+    of the tail 2.2, the fast exponential 4, the fast division 4 and its argument 2 times a slope of at most 2.7, eight steps of a sum whose
+    terms' magnitudes are at most twice the sum 16, three products 3; the exponent v^2 / 2 with its two products and constant 2.5 of itself: 42 + 1.3 v^2."""
+    v = torch.linspace(-8.0, 3.0, 264, device="cuda")
+    x, w = torch.zeros((rows, 64), dtype=F16, device="cuda"), _rand(264, 64, dtype=F16)
+    got = pkg.linear(x, w, v, activation="gelu", out_dtype=out_dtype)
+    want = (0.5 * v.double() * torch.special.erfc(-v.double() / 2 ** 0.5)).expand(rows, -1)
+    assert float(want[0, 0].abs()) < 6e-15
+    _check(got, want, (42 + 1.3 * v.double() ** 2) * U32 * want.abs())
