@@ -115,3 +115,14 @@ def test_gelu_keeps_its_negative_tail(pkg, rows, out_dtype):
     want = (0.5 * v.double() * torch.special.erfc(-v.double() / 2 ** 0.5)).expand(rows, -1)
     assert float(want[0, 0].abs()) < 6e-15
     _check(got, want, (42 + 1.3 * v.double() ** 2) * U32 * want.abs())
+
+
+@pytest.mark.parametrize("rows", [3, 60, 300])
+def test_softplus_is_relative_far_below_zero(pkg, rows):
+    """In half steps of fp32: the fast exponential 4, the fast division 4, the series and its sums 6; the exponential's argument v log2 e 1.25 of
+    itself (a product and the constant)."""
+    v = torch.cat([torch.linspace(-85.0, -10.0, 200), torch.linspace(-10.0, 4.0, 64), torch.tensor([-7.0, -20.0, -80.0, 0.0])]).cuda()
+    x, w = torch.zeros((rows, 64), dtype=F16, device="cuda"), _rand(v.numel(), 64, dtype=F16)
+    got = pkg.linear(x, w, v, activation="softplus", out_dtype=F32)
+    want = torch.log1p(torch.exp(v.double())).expand(rows, -1)
+    _check(got, want, (14 + 1.25 * v.double().clamp(max=0).abs()) * U32 * want)
