@@ -345,7 +345,7 @@ __device__ __forceinline__ void settle() {
 
 struct LinearMaps { CUtensorMap x, w; };
 struct LinearPlan {
-  int bn;            // MMA columns: rows of x (tile kernel), channels (pair kernel)
+  int bn;            // MMA columns: rows of x (tile kernel), channels (pair kernel: 64 at least, 32 for each half of its finishing warps)
   int stages, split;
   int m_tiles, n_tiles;
   int vec;           // out and residual rows can be taken four elements at a time (tile kernel) / eight (pair kernel)
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
       tc_fence_after();
       const uint32_t tm = tmem + (uint32_t)buf * 256 + ((uint32_t)(quad * 32) << 16);
       uint32_t acc[32];
-      if (32 * half < p.bn) tmem_ask32(tm + 32 * half, acc);
+      tmem_ask32(tm + 32 * half, acc);
       for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
         // 32 rows x 32 channels: the lane's row, bias and activation; through shared memory (16 bytes of a row where the row turns them, so that
         // neither side meets itself in a bank) to 8 channels of 8 rows at a time; the residual; out
@@ -691,9 +691,6 @@ __global__ void __launch_bounds__(LP_THREADS, 1) linear_pair_kernel(const Linear
             }
         }
         __syncwarp();
-      }
-      if (32 * half >= p.bn) {   // (32 channels: the other half's)
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
       }
     }
   }
