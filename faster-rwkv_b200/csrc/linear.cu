@@ -908,13 +908,15 @@ int fr_b200_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, int d
   OP_REQUIRE(x && w && out, "null tensor");
   const int es = dt_bytes(dtype), os = dt_bytes(out_dtype);
   OP_REQUIRE(aligned(x, es) && aligned(w, es) && aligned(out, os) && aligned(residual, os) && aligned(bias, 4), "misaligned pointer");
-  const Rows ro{out, ldo * os, (int64_t)N * os, rows};
-  OP_REQUIRE(!overlap(ro, Rows{x, ldx * es, (int64_t)K * es, rows}) && !overlap(ro, Rows{w, ldw * es, (int64_t)K * es, N}), "out overlaps x or w");
-  OP_REQUIRE(!overlap(ro, Rows{bias, 4 * (int64_t)N, 4 * (int64_t)N, bias ? 1 : 0}), "out overlaps the bias");
-  OP_REQUIRE((residual == out && ldr == ldo) || !overlap(ro, Rows{residual, ldr * os, (int64_t)N * os, residual ? rows : 0}),
+  const Rows ro{out, ldo * os, (int64_t)N * os, rows}, rx{x, ldx * es, (int64_t)K * es, rows}, rw{w, ldw * es, (int64_t)K * es, N},
+      rr{residual, ldr * os, (int64_t)N * os, residual ? rows : 0};
+  OP_REQUIRE(!overlap(ro, rx) && !overlap(ro, rw), "out overlaps x or w");
+  OP_REQUIRE(!overlap(ro, piece(bias, N, 4)), "out overlaps the bias");
+  OP_REQUIRE((residual == out && ldr == ldo) || !overlap(ro, rr),
              "the residual overlaps out without being it");
   const size_t need = fr_b200_linear_workspace(x, ldx, w, ldw, rows, K, N);
   OP_REQUIRE(!work || (aligned(work, 16) && work_bytes >= need), "the work area is smaller than fr_b200_linear_workspace() or not at 16 bytes");
+  for (const Rows &r : {ro, rx, rw, rr, piece(bias, N, 4)}) OP_REQUIRE(!overlap(r, piece(work, (int64_t)need, 1)), "the work area overlaps another argument");
   DeviceScope dev;
   OP_CU(dev.enter(device));
   LinearArgs a{x, w, residual, bias, out, ldx, ldw, ldr, ldo, (int)rows, N, K, act, out_dtype == FR_B200_T_F32};

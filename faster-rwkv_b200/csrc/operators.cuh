@@ -163,13 +163,16 @@ struct Rows {
   uintptr_t first() const { return reinterpret_cast<uintptr_t>(p); }
   uintptr_t end() const { return first() + (uintptr_t)((rows - 1) * ld + width); }
 };
-// Whether two pieces can have a byte in common: columns of the same rows do not.
+// `n` elements of `size` bytes one behind the other, or nothing
+inline Rows piece(const void *p, int64_t n, int64_t size) { return Rows{p, n * size, n * size, p && n > 0 ? 1 : 0}; }
+// Whether two pieces can have a byte in common: columns of the same rows do not, nor does a single row between two of the other's.
 inline bool overlap(const Rows &a, const Rows &b) {
   if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
   if (a.end() <= b.first() || b.end() <= a.first()) return false;
-  if (a.ld != b.ld || a.ld <= 0) return true;
-  const int64_t d = (int64_t)((b.first() % (uintptr_t)a.ld + (uintptr_t)a.ld - a.first() % (uintptr_t)a.ld) % (uintptr_t)a.ld);
-  return !(d >= a.width && d + b.width <= a.ld);
+  const int64_t ld = a.rows > 1 ? a.ld : b.ld;
+  if ((a.rows == 1 && b.rows == 1) || (b.rows > 1 && b.ld != ld) || ld <= 0) return true;
+  const int64_t d = (int64_t)((b.first() % (uintptr_t)ld + (uintptr_t)ld - a.first() % (uintptr_t)ld) % (uintptr_t)ld);
+  return !(d >= a.width && d + b.width <= ld);
 }
 
 // from / to of n streams over a pool of n_slots: nullptr: stream i has slot i.  -1: begins from zero / is not kept.  A slot is written by

@@ -258,6 +258,7 @@ int conv_check(const void *x, int64_t ldx, int dtype, int64_t rows, int D, const
   const Rows rs{state, state_stride * es, (int64_t)(taps - 1) * D * es, state ? n_slots : 0};
   OP_REQUIRE(!overlap(rx, ro), "out overlaps x");
   OP_REQUIRE(!overlap(rx, rs) && !overlap(ro, rs), "the pool of states overlaps x or out");
+  for (const Rows &r : {piece(w, (int64_t)D * taps, 4), piece(bias, D, 4)}) OP_REQUIRE(!overlap(r, ro) && !overlap(r, rs), "out or the pool of states overlaps a parameter");
   *a = {x, out, state, w, bias, ldx, ldo, state_stride, D, act == FR_B200_ACT_SILU};
   const size_t v = 4 * es;
   *vec = aligned(x, v) && aligned(out, v) && aligned(state, v) && aligned(w, 16) && aligned(bias, 16) && ldx % 4 == 0 && ldo % 4 == 0 && state_stride % 4 == 0 && D % 4 == 0;
@@ -368,7 +369,7 @@ cudaError_t ssm_step_any(const SsmArgs &a, const SlotTable &t, cudaStream_t st) 
 
 constexpr int SSM_STATES = 128;   // most states of a channel
 
-int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots) {
+int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots, size_t work_bytes) {
   OP_REQUIRE(dt_known(dtype), "dtype must be f16, bf16 or f32");
   OP_REQUIRE(rows >= 0 && rows < (1ll << 31) && a.d >= 1 && a.d <= (1 << 23), "bad shape");
   OP_REQUIRE(a.n >= 1 && a.n <= SSM_STATES, "1 to 128 states a channel");
@@ -387,6 +388,11 @@ int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots) {
                      {a.B, a.ldb * es, bn * es, rows}, {a.C, a.ldc * es, bn * es, rows}};
   for (const Rows &r : in) OP_REQUIRE(!overlap(out, r) && !overlap(pool, r), "out or the pool of states overlaps an input");
   OP_REQUIRE(!overlap(out, pool), "out overlaps the pool of states");
+  const Rows work = piece(a.work, (int64_t)work_bytes, 1), params[] = {piece(a.A, (int64_t)a.d * a.n, 4), piece(a.D, a.d, 4), piece(a.dt_bias, a.d, 4)};
+  for (const Rows &r : params) OP_REQUIRE(!overlap(r, out) && !overlap(r, pool), "out or the pool of states overlaps a parameter");
+  for (const Rows &r : params) OP_REQUIRE(!overlap(r, work), "the work area overlaps another argument");
+  for (const Rows &r : in) OP_REQUIRE(!overlap(r, work), "the work area overlaps another argument");
+  OP_REQUIRE(!overlap(out, work) && !overlap(pool, work), "the work area overlaps another argument");
   return FR_B200_OK;
 }
 
@@ -620,14 +626,14 @@ int fr_b200_ssm_seq(const void *x, int64_t ldx, const void *dt, int64_t lddt, co
   SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, reinterpret_cast<float *>(work), ldx, lddt, ldb, ldc, ldz, ldo, state_stride,
             D, N, groups, dt_softplus != 0, 0, 0};
   int rc;
-  if ((rc = ssm_check(a, dtype, rows, n_slots))) return rc;
+  const size_t need = fr_b200_ssm_seq_workspace(rows, n_seq, D, N);
+  if ((rc = ssm_check(a, dtype, rows, n_slots, need))) return rc;
   if ((rc = check_starts(starts, n_seq, rows)) || (rc = check_slots(n_seq, state, n_slots, from, to))) return rc;
   if (n_seq == 0) return FR_B200_OK;
   const size_t v = 8 * (size_t)dt_bytes(dtype);   // a thread's piece of a row: up to eight channels
   a.vec = aligned(x, v) && aligned(dt, v) && aligned(z, v) && aligned(out, v) && ldx % 8 == 0 && lddt % 8 == 0 && (!z || ldz % 8 == 0) && ldo % 8 == 0 &&
           (D / groups) % 8 == 0;
   a.shift = rows > 0 ? ssm_split(rows, n_seq, D) : 0;
-  const size_t need = fr_b200_ssm_seq_workspace(rows, n_seq, D, N);
   OP_REQUIRE(work_bytes >= need && (!need || (work && aligned(work, 4))), "the work area is smaller than fr_b200_ssm_seq_workspace()");
   DeviceScope dev;
   OP_CU(dev.enter(device));
@@ -650,7 +656,7 @@ int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, c
   OP_TRY
   SsmArgs a{x, dt, B, C, z, out, A, Dskip, dt_bias, state, nullptr, ldx, lddt, ldb, ldc, ldz, ldo, state_stride, D, N, groups, dt_softplus != 0, 0, 0};
   int rc;
-  if ((rc = ssm_check(a, dtype, n, n_slots)) || (rc = check_slots(n, state, n_slots, from, to))) return rc;
+  if ((rc = ssm_check(a, dtype, n, n_slots, 0)) || (rc = check_slots(n, state, n_slots, from, to))) return rc;
   a.vec = aligned(state, 16) && aligned(A, 16) && state_stride % 4 == 0 && N % 4 == 0;
   DeviceScope dev;
   OP_CU(dev.enter(device));

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_layer_ops_cpu import BF16, F32, O, R, S, W, X, _conv, _linear, _refused, _ssm
+
 
 def test_status_of_the_operators_without_a_device(pkg):
     L = pkg.lib()
@@ -13,3 +15,47 @@ def test_status_of_the_operators_without_a_device(pkg):
         assert L.fr_b200_op_status(0) == -3
         with pytest.raises(pkg.FrB200Error):
             pkg.check_operators()
+
+
+# ---- what may not overlap ----------------------------------------------------------------------------------------
+# conv: w [64, 4] and a bias of 64, out [20, 64] f16, a pool of 4 slots of 192; ssm: A [64, 16], D and dt_bias of 64, a pool of 4 of 1024 fp32
+
+@pytest.mark.parametrize("kw", [dict(w=O), dict(w=O + 20 * 128 - 4), dict(w=O - 64 * 4 * 4 + 4), dict(bias=O + 64), dict(w=S), dict(bias=S + 4 * 384 - 4), dict(bias=S - 252)])
+def test_conv_refuses_results_over_parameters(pkg, kw):
+    _refused(pkg, "fr_b200_conv_seq", _conv(**kw), "parameter")
+
+
+@pytest.mark.parametrize("seq", [True, False])
+@pytest.mark.parametrize("kw", [dict(A=O), dict(A=S + 4), dict(D=O + 124), dict(D=S), dict(bias=O), dict(bias=S + 4 * 4096 - 4), dict(A=O - 64 * 16 * 4 + 4)])
+def test_ssm_refuses_results_over_parameters(pkg, kw, seq):
+    _refused(pkg, "fr_b200_ssm_seq" if seq else "fr_b200_ssm_step", _ssm(seq, **kw), "parameter")
+
+
+def test_work_areas_overlap_nothing(pkg):
+    L = pkg.lib()
+    need = L.fr_b200_ssm_seq_workspace(2000, 1, 64, 16)
+    far = 0x70000000
+    assert need > 0
+    a = dict(rows=2000, work=far, wb=need, D=W + 0x100000, bias=W + 0x200000)
+    for at in (X, X + 0x1000000, X + 0x2000000, X + 0x3000000, W, W + 0x100000, W + 0x200000, S, O):
+        _refused(pkg, "fr_b200_ssm_seq", _ssm(**{**a, "work": at}), "work area")
+        _refused(pkg, "fr_b200_ssm_seq", _ssm(**{**a, "work": at - need + 4}), "work area")
+    a = dict(rows=4000, K=1001, ldx=1001, ldw=1001, N=100, ldo=100, work_bytes=4100 * 126 * 16, bias=far, residual=R, ldr=100)
+    for at in (X, W, O, R, far):
+        _refused(pkg, "fr_b200_linear", _linear(**a, work=at), "work area")
+    if not torch.cuda.is_available():     # (no device: past the checks)
+        assert L.fr_b200_linear(*_linear(**a, work=far + 0x1000)) == -3
+        assert L.fr_b200_ssm_seq(*_ssm(rows=2000, work=far, wb=need)) == -3
+
+
+def test_a_parameter_between_rows_does_not_overlap(pkg):
+    """rows far apart, with the parameters in what lies between them: taken as before"""
+    if torch.cuda.is_available():
+        pytest.skip("GPU present: the addresses are not memory")
+    L = pkg.lib()
+    assert L.fr_b200_conv_seq(*_conv(out=O, ldo=4096, w=O + 128, bias=O + 128 + 1024)) == -3
+    _refused(pkg, "fr_b200_conv_seq", _conv(out=O, ldo=4096, w=O + 124), "parameter")
+    _refused(pkg, "fr_b200_conv_seq", _conv(out=O, ldo=4096, bias=O + 8192 - 252), "parameter")
+    assert L.fr_b200_linear(*_linear(out=O, ldo=512, bias=O + 64)) == -3
+    _refused(pkg, "fr_b200_linear", _linear(out=O, ldo=512, bias=O + 60), "bias")
+    assert L.fr_b200_linear(*_linear(dtype=BF16, out_dtype=F32, rows=1, x=O + 128)) == -3
