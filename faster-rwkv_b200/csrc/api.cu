@@ -1542,14 +1542,19 @@ int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   try {
     if (int rc = check_moves(m->cfg.max_batch, n, src, dst)) return fail(rc, fr_b200_op_last_error());
-    if (capturing(st)) return fail(FR_B200_E_STATE, "state_copy on a capturing stream: which copy of its token-shift states a slot reads is kept on the host");
+    if (capturing(st)) return fail(FR_B200_E_STATE, "state_copy on a capturing stream: which copy of its token-shift states a slot reads is known to the host, and changes from token to token");
     CU(cudaSetDevice(m->device));
-    // both copies of the token-shift states move, and with them which one is read next
-    std::vector<unsigned> par(m->par);
+    // Both copies of the token-shift states move.  Which of them a slot's next token reads stays as it is (steps captured before go on reading
+    // that one): where the source reads the other, its copy is taken over.
+    std::vector<int32_t> turned;
+    std::vector<uint8_t> reads;
+    for (int i = 0; i < n; ++i)
+      if (src[i] >= 0 && m->par[src[i]] != m->par[dst[i]]) { turned.push_back(dst[i]); reads.push_back((uint8_t)m->par[dst[i]]); }
     const SlotFill pp{off_mid(m->C, m->cfg.act_fp16) + 2 * (size_t)m->C * 4, m->layer_stride, m->L, m->C, -1e30f};
     CU(launch_slots_copy(m->d_state, m->layer_stride * m->L, m->state_stride, m->cfg.max_batch, n, src, dst, m->v5 ? nullptr : &pp, st));
-    for (int i = 0; i < n; ++i) par[dst[i]] = src[i] < 0 ? 0u : m->par[src[i]];
-    m->par.swap(par);
+    const int af = m->cfg.act_fp16;
+    const SlotPairs shift{{off_sx(m->C, af, 0), off_ffn_sx(m->C, m->H, m->v5, af, 0)}, m->layer_stride, m->L, (int)(m->C * act_bytes(af) / 4)};
+    CU(launch_slots_turn(m->d_state, m->state_stride, (int)turned.size(), turned.data(), reads.data(), shift, st));
     if (m->cfg.host_visible_state) CU(cudaStreamSynchronize(st));
   } catch (const std::bad_alloc &) {
     return fail(FR_B200_E_NOMEM, "out of host memory");

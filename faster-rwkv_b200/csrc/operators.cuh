@@ -186,6 +186,11 @@ struct SlotFill { size_t offset, layer_stride; int layers, n; float value; };
 cudaError_t launch_slots_copy(void *pool, size_t bytes, size_t stride, int n_slots, int n, const int32_t *src, const int32_t *dst,
                               const SlotFill *fill, cudaStream_t st);
 
+// two vectors of `words` 32-bit words that every layer of a slot holds twice, the second copy of each behind the first
+struct SlotPairs { size_t offset[2], layer_stride; int layers, words; };
+// in each of n slots the copies 1 - to[i] of its vectors to their copies to[i]
+cudaError_t launch_slots_turn(void *pool, size_t stride, int n, const int32_t *slots, const uint8_t *to, const SlotPairs &p, cudaStream_t st);
+
 // Sequences of one launch, by value: a captured graph holds them, as it holds the ids of a decode step.
 constexpr int SEQ_CAP = 256;
 struct SeqTable {

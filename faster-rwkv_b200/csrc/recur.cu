@@ -528,6 +528,17 @@ __global__ void __launch_bounds__(COPY_THREADS) slots_fill_kernel(uint8_t *at, s
   if (e < n && t.from[blockIdx.z] == t.n_src) reinterpret_cast<float *>(at + t.dst[blockIdx.z] * stride + blockIdx.y * layer_stride)[e] = value;
 }
 
+constexpr int TURN_CAP = 256;
+struct TurnTable { uint16_t slot[TURN_CAP]; uint8_t to[TURN_CAP]; };
+__global__ void __launch_bounds__(COPY_THREADS) slots_turn_kernel(uint8_t *pool, size_t stride, const SlotPairs p, const __grid_constant__ TurnTable t) {
+  const int e = blockIdx.x * COPY_THREADS + threadIdx.x, which = blockIdx.y & 1;
+  pdl_wait();
+  pdl_trigger();
+  uint32_t *v = reinterpret_cast<uint32_t *>(pool + t.slot[blockIdx.z] * stride + (blockIdx.y >> 1) * p.layer_stride + (which ? p.offset[1] : p.offset[0]));
+  const int to = t.to[blockIdx.z];
+  if (e < p.words) v[to * p.words + e] = v[(1 - to) * p.words + e];
+}
+
 template <int CAP>
 cudaError_t slots_copy_moves(uint8_t *pool, size_t bytes, size_t stride, int n_slots, int n, const int32_t *src, const int32_t *dst, const SlotFill *fill,
                              cudaStream_t st) {
@@ -572,6 +583,18 @@ cudaError_t frb::launch_slots_copy(void *pool, size_t bytes, size_t stride, int 
   uint8_t *p = reinterpret_cast<uint8_t *>(pool);
   if (n <= COPY_SMALL) return slots_copy_moves<COPY_SMALL>(p, bytes, stride, n_slots, n, src, dst, fill, st);
   return slots_copy_moves<COPY_CAP>(p, bytes, stride, n_slots, n, src, dst, fill, st);
+}
+
+cudaError_t frb::launch_slots_turn(void *pool, size_t stride, int n, const int32_t *slots, const uint8_t *to, const SlotPairs &p, cudaStream_t st) {
+  for (int i0 = 0; i0 < n; i0 += TURN_CAP) {
+    TurnTable t;
+    const int m = std::min(n - i0, TURN_CAP);
+    for (int i = 0; i < m; ++i) { t.slot[i] = (uint16_t)slots[i0 + i]; t.to[i] = to[i0 + i]; }
+    const cudaError_t e = op_launch(slots_turn_kernel, dim3((p.words + COPY_THREADS - 1) / COPY_THREADS, 2 * p.layers, m), COPY_THREADS, 0, st, 1,
+                                    reinterpret_cast<uint8_t *>(pool), stride, p, t);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 extern "C" {

@@ -338,7 +338,8 @@ int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, c
 int fr_b200_slots_copy(void *pool, size_t slot_bytes, size_t slot_stride, int n_slots, int n, const int32_t *src, const int32_t *dst, int device,
                        void *stream);
 /* The same for the state slots of a model (fork a prompt's state into several streams, close the gaps that finished streams leave); src -1:
- * the initial state of fr_b200_state_reset.  Ordered on `stream` like the model's other calls; not on a capturing stream (FR_B200_E_STATE). */
+ * the initial state of fr_b200_state_reset.  Ordered on `stream` like the model's other calls; steps that were captured before go on from the
+ * new states.  Not on a capturing stream (FR_B200_E_STATE). */
 int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_t *dst, void *stream);
 
 

@@ -1,8 +1,11 @@
 """Edges of the operators of a recurrent layer: calls that their documentation allows and that lie beside the ordinary ones."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
+from test_gpu_batch import _capture
 from test_gpu_layer_ops import BF16, EX2, F16, F32, U32, _check, _linear_want, _rand, _ssm_inputs, _ssm_want
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +129,37 @@ def test_softplus_is_relative_far_below_zero(pkg, rows):
     got = pkg.linear(x, w, v, activation="softplus", out_dtype=F32)
     want = torch.log1p(torch.exp(v.double())).expand(rows, -1)
     _check(got, want, (14 + 1.25 * v.double().clamp(max=0).abs()) * U32 * want)
+
+
+# ---- states of a model -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("version,fmt", [("4", "cuda fp16"), ("4", "cuda int8"), ("5.2", "cuda fp16")])
+def test_captured_steps_go_on_from_copied_states(pkg, synth, version, fmt):
+    """Two tokens of two streams as a graph.  Between its replays their slots take states of streams that have seen one token more or less: a token reads
+    one of two copies of the token-shift states, the graph always the same one."""
+    shape = synth.Shape(version, 2, 128, 512, 96, n_head=2 if version != "4" else 0)
+    tensors = synth.to_file_dtypes(shape, synth.generate(shape, seed=11, ln_random=True), "fp16" if fmt.endswith("fp16") else "fp32")
+    m = pkg.Model(tensors, fmt, shape=shape, max_batch=6)
+    ids = synth.token_ids(shape, 4, seed=9).reshape(2, 2).astype(np.int32)
+    m.run([5])                                          # stream 0: one token, the others none
+    m.copy_states([0], [4])
+    m.run([9])
+    m.copy_states([0, 0], [5, 3])                       # 4: one token, 5 and 3: two
+    assert np.array_equal(m.export_state(5), m.export_state(0)) and np.array_equal(m.export_state(3), m.export_state(0))
+    kept = {b: m.export_state(b) for b in (3, 4, 5)}
+    m.copy_states([-1, -1], [0, 1])
+    got = torch.zeros(2, 2, shape.vocab, device="cuda")
+    graph = _capture(pkg, lambda st: [pkg.lib().fr_b200_decode(m.handle, ids[t].ctypes.data_as(ctypes.c_void_p), 2,
+                                                               ctypes.c_void_p(got[t].data_ptr()), None, st) for t in (0, 1)])
+    for pair in ((4, 5), (5, 4), (4, 4), (3, -1), (-1, 4)):
+        for b in (0, 1):                                # what the same states give outside the graph, stream by stream
+            m.import_state(kept[pair[b]] if pair[b] >= 0 else m.export_state(2), b)
+        want = np.stack([m.decode(ids[t]) for t in (0, 1)])
+        after = [m.export_state(b) for b in (0, 1)]
+        m.copy_states(list(pair), [0, 1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(got.cpu().numpy(), want), pair
+        assert all(np.array_equal(m.export_state(b), after[b]) for b in (0, 1)), pair
+        assert all(np.array_equal(m.export_state(b), k) for b, k in kept.items())
+    m.close()
