@@ -151,6 +151,15 @@ def parse_strategy(strategy: str):
     return fmt, 1 if fmt == W_FP16 else 0
 
 
+def _slot_list(v, what: str) -> np.ndarray:
+    a = np.asarray(v)
+    if a.ndim != 1 or (a.size and a.dtype.kind not in "iu"):
+        raise ValueError(f"{what} is not a list of integers")
+    if a.size and (int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
+        raise ValueError(f"{what} has an entry that is no 32-bit integer")
+    return np.ascontiguousarray(a, np.int32)
+
+
 class Model:
     """rwkv::Model on the B200 backend.  `max_batch` > 1 adds the batched decode the reference lacks."""
 
@@ -274,8 +283,8 @@ class Model:
         """Slot dst[i] takes the state that slot src[i] has before the call (src -1: the initial state), on the device:
         fork a prompt's state into several streams, reorder the streams of a beam search, close the gaps that finished
         streams leave.  Every slot appears in dst once at most."""
-        s, d = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
-        if s.shape != d.shape or s.ndim != 1:
+        s, d = _slot_list(src, "src"), _slot_list(dst, "dst")
+        if len(s) != len(d):
             raise ValueError("src and dst are two lists of as many slots")
         check(lib().fr_b200_state_copy(self._h, len(s), _np_ptr(s), _np_ptr(d), None), "fr_b200_state_copy")
 

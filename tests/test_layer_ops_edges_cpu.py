@@ -1,4 +1,5 @@
 """Edges of the operators of a recurrent layer that need no device: refusals, status codes, arguments."""
+import numpy as np
 import pytest
 import torch
 
@@ -59,3 +60,18 @@ def test_a_parameter_between_rows_does_not_overlap(pkg):
     assert L.fr_b200_linear(*_linear(out=O, ldo=512, bias=O + 64)) == -3
     _refused(pkg, "fr_b200_linear", _linear(out=O, ldo=512, bias=O + 60), "bias")
     assert L.fr_b200_linear(*_linear(dtype=BF16, out_dtype=F32, rows=1, x=O + 128)) == -3
+
+
+# ---- lists of slots ----------------------------------------------------------------------------------------------
+
+def test_model_copy_states_takes_whole_numbers_alone(pkg):
+    """what is no 32-bit integer is refused, not cut down to one"""
+    m = object.__new__(pkg.Model)
+    m._h = None
+    for src, dst in (([0.5], [1]), ([0], [1.9]), (np.array([2 ** 32]), [1]), ([0], np.array([2 ** 32 + 1])), ([-2 ** 40], [0]), (np.array([2 ** 63], np.uint64), [0]),
+                     (["0"], ["1"]), ([True], [False]), ([[0]], [[1]]), (0, 1), ([0, 1], [1]), (np.array([2 ** 31]), [0])):
+        with pytest.raises(ValueError):
+            m.copy_states(src, dst)
+    for src, dst in (([0], [1]), ((0, 2), np.array([1, 3], np.int64)), ([], []), (np.array([-1], np.int8), [5])):
+        with pytest.raises(pkg.FrB200Error):       # taken: the library refuses the model that is not there
+            m.copy_states(src, dst)
