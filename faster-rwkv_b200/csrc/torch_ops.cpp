@@ -298,6 +298,7 @@ PyObject *py_ssm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     from.take(a[10], streams, "from_slots", true);
     to.take(a[11], streams, "to_slots", true);
     const int softplus = PyObject_IsTrue(a[8]);
+    if (softplus < 0) throw Bad{};
     const int di = fit(d, "x"), ni = fit(states, "A"), gi = fit(groups, "B");
     const Place at(x);
     if (!seq)

@@ -163,3 +163,17 @@ def test_captured_steps_go_on_from_copied_states(pkg, synth, version, fmt):
         assert all(np.array_equal(m.export_state(b), after[b]) for b in (0, 1)), pair
         assert all(np.array_equal(m.export_state(b), k) for b, k in kept.items())
     m.close()
+
+
+# ---- arguments ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("call", ["ssm_seq", "ssm_step"])
+def test_dt_softplus_without_a_truth_value(pkg, call):
+    """what cannot be asked for its truth raises what it raises, and nothing is launched"""
+    x, dt, A, B, C, *_ = _ssm_inputs(4, 8, 2, 1, F16)
+    out = torch.full((4, 8), 7.0, dtype=F16, device="cuda")
+    with pytest.raises(ValueError, match="ambiguous"):
+        getattr(pkg, call)(x, dt, A, B, C, dt_softplus=np.array([1, 2]), out=out)
+    assert bool((out == 7).all())
+    for yes in (True, 1, np.bool_(True), torch.tensor(True)):
+        assert torch.equal(getattr(pkg, call)(x, dt, A, B, C, dt_softplus=yes), getattr(pkg, call)(x, dt, A, B, C))
