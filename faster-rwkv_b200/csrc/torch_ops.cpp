@@ -4,6 +4,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Dtype.h>
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 
@@ -34,7 +35,9 @@ struct Bad {};   // a Python error is set
 const at::Tensor *tensor(PyObject *o, const char *what) {
   if (o == Py_None) return nullptr;
   if (!THPVariable_Check(o)) bad("%s is not a tensor", what);
-  return &THPVariable_Unpack(o);
+  const at::Tensor &t = THPVariable_Unpack(o);
+  if (t.requires_grad() && c10::GradMode::is_enabled()) bad("%s requires a gradient, and none flows through this operator: call it under torch.no_grad()", what);
+  return &t;
 }
 const at::Tensor &needed(PyObject *o, const char *what) {
   const at::Tensor *t = tensor(o, what);

@@ -2,7 +2,8 @@
 fr_b200_slots_copy on the tensors' device and torch's current stream, through csrc/fr_b200_torch.so.
 
 Tensors are [rows, width] with adjacent elements and any distance between rows, so that pieces of a wider projection go in as
-they are; they are not copied or cast.  Results are new tensors unless `out` is given; no gradient flows through them.
+they are; they are not copied or cast.  Results are new tensors unless `out` is given.  No gradient flows through them: a tensor that requires one is
+refused outside torch.no_grad() and torch.inference_mode().
 Sequences (`starts`) and slots are host lists, numpy int32 arrays or CPU integer tensors; a call that is captured into a CUDA
 graph holds them by value.  ValueError: tensors that do not fit together; FrB200Error: what the library refuses.
 """

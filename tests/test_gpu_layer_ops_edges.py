@@ -177,3 +177,16 @@ def test_dt_softplus_without_a_truth_value(pkg, call):
     assert bool((out == 7).all())
     for yes in (True, 1, np.bool_(True), torch.tensor(True)):
         assert torch.equal(getattr(pkg, call)(x, dt, A, B, C, dt_softplus=yes), getattr(pkg, call)(x, dt, A, B, C))
+
+
+def test_parameters_without_gradients(pkg):
+    """weights that require a gradient: taken under no_grad, refused in every place outside it"""
+    x, w, b = _rand(4, 64, dtype=F16), _rand(24, 64, dtype=F16, scale=0.1, seed=1), _rand(24, seed=2)
+    want = pkg.linear(x, w, b)
+    wp, bp = torch.nn.Parameter(w.clone()), torch.nn.Parameter(b.clone())
+    with torch.no_grad():
+        assert torch.equal(pkg.linear(x, wp, bp), want)
+    assert torch.equal(pkg.linear(x, wp.detach(), bp.detach()), want)
+    for args, kw in (((x, wp, b), {}), ((x, w, bp), {}), ((x, w, b), {"residual": want.clone().requires_grad_()}), ((x.clone().requires_grad_(), w, b), {})):
+        with pytest.raises(ValueError, match="gradient"):
+            pkg.linear(*args, **kw)

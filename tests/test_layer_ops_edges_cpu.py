@@ -75,3 +75,19 @@ def test_model_copy_states_takes_whole_numbers_alone(pkg):
     for src, dst in (([0], [1]), ((0, 2), np.array([1, 3], np.int64)), ([], []), (np.array([-1], np.int8), [5])):
         with pytest.raises(pkg.FrB200Error):       # taken: the library refuses the model that is not there
             m.copy_states(src, dst)
+
+
+# ---- gradients ---------------------------------------------------------------------------------------------------
+
+def test_tensors_that_require_a_gradient(pkg):
+    """no gradient flows: said before anything else, instead of a result that has none.  Under no_grad and inference_mode they are taken (and
+    refused here for their place, the CPU)."""
+    x, p = torch.zeros(4, 8), torch.nn.Parameter(torch.zeros(8, 8))
+    calls = [lambda: pkg.linear(p, x), lambda: pkg.linear(x, p), lambda: pkg.conv_step(p, x), lambda: pkg.conv_seq(x, p), lambda: pkg.ssm_step(x, x, p, x, x),
+             lambda: pkg.ssm_seq(p, x, x, x, x), lambda: pkg.copy_slots(p, [0], [1])]
+    for f in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            f()
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode(), pytest.raises(ValueError, match="GPU"):
+                f()
