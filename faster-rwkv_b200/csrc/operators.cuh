@@ -21,6 +21,7 @@ namespace frb {
 
 // status + text for fr_b200_op_last_error()
 int op_fail(int code, const std::string &msg);
+int op_caught(int code, const char *what) noexcept;   // (`what` short enough for a string that allocates nothing)
 #define OP_CU(call)                                                                                               \
   do {                                                                                                            \
     cudaError_t e_ = (call);                                                                                      \
@@ -34,8 +35,8 @@ int op_fail(int code, const std::string &msg);
 #define OP_TRY try {
 #define OP_CATCH                                                                          \
   }                                                                                       \
-  catch (const std::bad_alloc &) { return FR_B200_E_NOMEM; }                              \
-  catch (...) { return FR_B200_E_ARG; }
+  catch (const std::bad_alloc &) { return frb::op_caught(FR_B200_E_NOMEM, "out of memory"); } \
+  catch (...) { return frb::op_caught(FR_B200_E_ARG, "an exception"); }
 
 // The call's device is current inside the call and the caller's again behind it.
 struct DeviceScope {

@@ -16,6 +16,11 @@ namespace {
 thread_local std::string g_op_err;
 }
 int frb::op_fail(int code, const std::string &msg) { g_op_err = msg; return code; }
+int frb::op_caught(int code, const char *what) noexcept {
+  g_op_err.clear();
+  g_op_err.append(what);
+  return code;
+}
 
 namespace {
 

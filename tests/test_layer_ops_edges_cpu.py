@@ -1,4 +1,8 @@
 """Edges of the operators of a recurrent layer that need no device: refusals, status codes, arguments."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -91,3 +95,30 @@ def test_tensors_that_require_a_gradient(pkg):
         for mode in (torch.no_grad, torch.inference_mode):
             with mode(), pytest.raises(ValueError, match="GPU"):
                 f()
+
+
+# ---- out of memory -----------------------------------------------------------------------------------------------
+
+NOMEM = """
+import resource
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import __graft_entry__ as entry
+from test_layer_ops_cpu import _conv, _i32
+pkg = entry.load_package()
+L = pkg.lib()
+assert L.fr_b200_conv_seq(*_conv(taps=9)) == -1
+with open("/proc/self/statm") as f:
+    held = int(f.read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (held + (1 << 30), resource.RLIM_INFINITY))
+# the record of who writes which slot would take 16 GB
+rc = L.fr_b200_conv_seq(*_conv(n_slots=2 ** 31 - 1, fro=_i32(0), to=_i32(1)))
+print(rc, L.fr_b200_op_last_error().decode())
+"""
+
+
+def test_host_memory_that_runs_out_has_its_own_text(pkg):
+    """no exception crosses the C interface, and the text is not that of the call before"""
+    tests = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", NOMEM.format(root=os.path.dirname(tests), tests=tests)], capture_output=True, text=True, timeout=300)
+    assert r.stdout == "-7 out of memory\n", (r.stdout, r.stderr[-500:])
