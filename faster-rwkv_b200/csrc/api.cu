@@ -100,7 +100,8 @@ struct fr_b200_model {
   float *d_lnvec = nullptr;           // ln_out of the last prompt token
   cudaStream_t seq_streams[4] = {nullptr, nullptr, nullptr, nullptr};   // long prompts: one stream per piece of rows
   std::vector<cudaEvent_t> seq_events;                                  // [piece][layer] + one start event
-  // buffers that were outgrown after a call on a capturing stream: its graph goes on using them (see grow())
+  // Once a step was captured: its graph goes on using the buffers that a later call outgrows (see grow()), and on reading the copy of the token-shift
+  // states that it was captured with (state_reset, state_copy).
   bool captured = false;
   std::vector<void *> outgrown;
   // scratch for uploads
@@ -817,6 +818,7 @@ static int decode_impl(fr_b200_model *m, const int32_t *ids_host, const unsigned
   // A captured launch keeps its tags at every replay, whatever ran before and whatever runs next: it clears the words on both
   // sides (with one layer every word of the replay before would pass for this one's).
   const bool replayed = capturing(st);
+  m->captured = m->captured || replayed;
   if (m->exch_batch != batch || replayed) CU(cudaMemsetAsync(m->d_exch, 0, m->exch_bytes, st));
   m->exch_batch = replayed ? 0 : batch;   // (nothing has run yet: the next launch starts clean)
   p.seq_base = 255u + m->seq;
@@ -1510,10 +1512,11 @@ int fr_b200_state_reset(fr_b200_model *m, int slot) {
       for (int i = 0; i < m->C; ++i) pp[i] = -1e30f;
     }
   }
+  // (both copies of the token-shift states begin anew, so that the next token may read either; steps captured before read theirs)
   for (int s = 0; s < m->cfg.max_batch; ++s)
     if (slot < 0 || slot == s) {
       CU(cudaMemcpy(m->d_state + (size_t)s * m->state_stride, h.data(), per, cudaMemcpyHostToDevice));
-      m->par[s] = 0;
+      if (!m->captured) m->par[s] = 0;
     }
   return FR_B200_OK;
 }
@@ -1544,17 +1547,21 @@ int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_
     if (int rc = check_moves(m->cfg.max_batch, n, src, dst)) return fail(rc, fr_b200_op_last_error());
     if (capturing(st)) return fail(FR_B200_E_STATE, "state_copy on a capturing stream: which copy of its token-shift states a slot reads is known to the host, and changes from token to token");
     CU(cudaSetDevice(m->device));
-    // Both copies of the token-shift states move.  Which of them a slot's next token reads stays as it is (steps captured before go on reading
-    // that one): where the source reads the other, its copy is taken over.
+    // Both copies of the token-shift states move, and with them which one is read next, so that streams forked from one are decoded together as they
+    // are.  Where steps were captured a slot goes on reading the copy that it read (they do): if the source reads the other one, that is copied over.
+    std::vector<unsigned> par(m->par);
     std::vector<int32_t> turned;
     std::vector<uint8_t> reads;
-    for (int i = 0; i < n; ++i)
-      if (src[i] >= 0 && m->par[src[i]] != m->par[dst[i]]) { turned.push_back(dst[i]); reads.push_back((uint8_t)m->par[dst[i]]); }
+    for (int i = 0; i < n; ++i) {
+      if (!m->captured) par[dst[i]] = src[i] < 0 ? 0u : m->par[src[i]];
+      else if (src[i] >= 0 && m->par[src[i]] != m->par[dst[i]]) { turned.push_back(dst[i]); reads.push_back((uint8_t)m->par[dst[i]]); }
+    }
     const SlotFill pp{off_mid(m->C, m->cfg.act_fp16) + 2 * (size_t)m->C * 4, m->layer_stride, m->L, m->C, -1e30f};
     CU(launch_slots_copy(m->d_state, m->layer_stride * m->L, m->state_stride, m->cfg.max_batch, n, src, dst, m->v5 ? nullptr : &pp, st));
     const int af = m->cfg.act_fp16;
     const SlotPairs shift{{off_sx(m->C, af, 0), off_ffn_sx(m->C, m->H, m->v5, af, 0)}, m->layer_stride, m->L, (int)(m->C * act_bytes(af) / 4)};
     CU(launch_slots_turn(m->d_state, m->state_stride, (int)turned.size(), turned.data(), reads.data(), shift, st));
+    m->par.swap(par);
     if (m->cfg.host_visible_state) CU(cudaStreamSynchronize(st));
   } catch (const std::bad_alloc &) {
     return fail(FR_B200_E_NOMEM, "out of host memory");
