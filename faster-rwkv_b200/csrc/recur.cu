@@ -698,6 +698,7 @@ int fr_b200_ssm_step(const void *x, int64_t ldx, const void *dt, int64_t lddt, c
 int fr_b200_slots_copy(void *pool, size_t slot_bytes, size_t slot_stride, int n_slots, int n, const int32_t *src, const int32_t *dst, int device,
                        void *stream) {
   OP_TRY
+  if (n == 0) return FR_B200_OK;
   OP_REQUIRE(pool && slot_bytes > 0 && slot_stride >= slot_bytes, "bad argument");
   int rc;
   if ((rc = check_moves(n_slots, n, src, dst))) return rc;

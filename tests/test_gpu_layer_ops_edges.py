@@ -26,6 +26,35 @@ def test_copy_slots_that_only_clears(pkg, dtype, row):
         assert torch.equal(p, want)
 
 
+def test_no_streams_and_no_rows(pkg):
+    """a step of a server without streams, and sequences without a row in rows that are none: states are handed on"""
+    e = lambda *s: torch.empty(s, dtype=F16, device="cuda")  # noqa: E731
+    w, A = _rand(16, 4), -torch.ones((16, 8), device="cuda")
+    conv, ssm = _rand(5, 3, 16, dtype=F16), _rand(5, 16, 8, seed=1)
+    for f, t in (([], []), (np.zeros(0, np.int32), ()), (torch.zeros(0, dtype=torch.int32), []), (-1, -1), (None, None)):
+        p, q = conv.clone(), ssm.clone()
+        assert pkg.conv_step(e(0, 16), w, state=p, from_slots=f, to_slots=t).shape == (0, 16)
+        assert pkg.ssm_step(e(0, 16), e(0, 16), A, e(0, 8), e(0, 8), state=q, from_slots=f, to_slots=t).shape == (0, 16)
+        assert pkg.conv_seq(e(0, 16), w, state=p, starts=[0], from_slots=f, to_slots=t).shape == (0, 16)
+        assert pkg.ssm_seq(e(0, 16), e(0, 16), A, e(0, 8), e(0, 8), state=q, starts=[0], from_slots=f, to_slots=t).shape == (0, 16)
+        assert torch.equal(p, conv) and torch.equal(q, ssm)
+    pkg.conv_seq(e(0, 16), w, state=p, starts=[0, 0, 0], from_slots=[1, -1], to_slots=[4, 2])
+    pkg.ssm_seq(e(0, 16), e(0, 16), A, e(0, 8), e(0, 8), state=q, starts=[0, 0, 0], from_slots=[1, -1], to_slots=[4, 2])
+    for new, old in ((p, conv), (q, ssm)):
+        assert torch.equal(new[4], old[1]) and bool((new[2] == 0).all()) and torch.equal(new[[0, 1, 3]], old[[0, 1, 3]])
+    for pool in (conv[:0], conv, conv[:, :0]):
+        assert pkg.copy_slots(pool, [], []) is pool
+
+
+@pytest.mark.parametrize("rows", [17, 40, 300, 2000])
+@pytest.mark.parametrize("k,n", [(8, 1), (64, 1), (8, 8), (1, 3), (16, 2)])
+def test_linear_of_the_smallest_matrices(pkg, rows, k, n):
+    """one channel, and inputs of one word: boxes of a tile that reach past all of the matrix"""
+    x, w = _rand(rows, k, dtype=F16), _rand(n, k, dtype=F16, seed=1)
+    want, err = _linear_want(x, w, None, "none", None)
+    _check(pkg.linear(x, w), want, err)
+
+
 # ---- waits that give up ------------------------------------------------------------------------------------------
 
 def test_a_wait_that_gave_up_is_told_once_and_refuses_nobody(pkg):

@@ -122,3 +122,10 @@ def test_host_memory_that_runs_out_has_its_own_text(pkg):
     tests = os.path.dirname(os.path.abspath(__file__))
     r = subprocess.run([sys.executable, "-c", NOMEM.format(root=os.path.dirname(tests), tests=tests)], capture_output=True, text=True, timeout=300)
     assert r.stdout == "-7 out of memory\n", (r.stdout, r.stderr[-500:])
+
+
+def test_no_moves_ask_for_nothing(pkg):
+    L = pkg.lib()
+    assert L.fr_b200_slots_copy(None, 0, 0, 0, 0, None, None, 0, None) == 0
+    assert L.fr_b200_slots_copy(S, 64, 64, 8, 0, None, None, 0, None) == 0
+    _refused(pkg, "fr_b200_slots_copy", (S, 64, 64, 8, -1, None, None, 0, None), "moves")
