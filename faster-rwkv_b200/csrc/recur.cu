@@ -79,9 +79,10 @@ void fill_slots(SlotTable &t, int i0, int n, const void *state, const int32_t *f
 
 // ---- the short causal convolution --------------------------------------------------------------------------------
 // y[t, d] = act(b[d] + sum_j w[d, j] x[t - (W - 1) + j, d]); what lies before a sequence's first row are the W - 1 rows of its state.
-// Bound by memory: x once, y once, for a few multiply-adds an element.  4001 rows of 5120 bf16 channels in 37 sequences, 82 MB: 22 us, 3.7 TB/s (a
-// copy of the same rows with torch 46); 8 rows a thread 27, 8 channels a thread 31.  Loads without a branch: what is not there is read from some
-// place that is, and not taken (24 us with branches).  One token of 64 streams of 4096 channels 2.5 us.
+// Bound by memory: x once, y once, for a few multiply-adds an element.  4001 rows of 5120 bf16 channels in 37 sequences, 82 MB: 22.8 us, 3.7 TB/s, of the
+// 6.55 that a copy of large buffers reaches (a CTA loads, waits, stores and ends: half of the issue slots are used, a quarter of the warps are there); 8 rows a thread 27,
+// 8 channels a thread 31.  Loads without a branch: what is not there is read from some place that is, and not taken (24 us with branches).  Rows off the 16-byte
+// boundaries 28 us, where rows on them take 17 in the same loop.  One token of 64 streams of 4096 channels 2.5 us.
 struct ConvArgs {
   const void *x;
   void *out, *state;
@@ -397,7 +398,7 @@ int ssm_check(SsmArgs &a, int dtype, int64_t rows, int n_slots, size_t work_byte
 }
 
 // Pieces of 2^shift rows, or 0: sequences whole.  Long sequences of few channels: their pieces side by side, twice the work, as long as that leaves a CTA
-// or two for every SM.  One of 4096 rows and 768 channels 80 us whole, 67 in pieces of 256 rows; of 256 channels 27 in pieces.
+// or two for every SM.  One of 4096 rows and 768 channels 79 us whole, 67 in pieces of 256 rows; of 256 channels 78 and 28.
 int ssm_split(int64_t rows, int n_seq, int d) {
   const int64_t units = (int64_t)((d + 31) / 32) * n_seq;
   if (units > 24 || rows < 1024ll * n_seq) return 0;

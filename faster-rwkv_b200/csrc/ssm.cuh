@@ -2,7 +2,8 @@
 // ssm_bf16.cu and ssm_f32.cu.
 //   delta = softplus(dt + dt_bias)      h[d, n] <- exp(delta[d] A[d, n]) h[d, n] + delta[d] x[d] B[g(d), n]
 //   y[d] = (sum_n C[g(d), n] h[d, n] + D[d] x[d]) * silu(z[d])           g(d) = d / (channels / groups)
-// Bound by the exponentials: one for each row, channel and state, 16 a clock and SM, and four more for softplus and silu.
+// Its floor are the exponentials: one for each row, channel and state, 16 a clock and SM, and four more for softplus and silu.  It takes 1.7 to 2.3 times
+// as long; what holds it up stands below.
 #pragma once
 #include "operators.cuh"
 
@@ -29,8 +30,9 @@ template <typename T> cudaError_t launch_ssm_seq(const SsmArgs &a, const SeqTabl
 // Everything lies in shared memory along the rows: a lane takes four rows of a state with loads of 16 bytes, packed products of neighbouring rows and
 // one multiply-add a row.  The sums over a channel's lanes are taken L rows at a time, so that every lane ends with one row's (L - 1
 // shuffles for L rows).
-// What bounds it: with work for all SMs the words that lanes load from shared memory, 2 L + 32 a row of 32 channels (16 states), next to 40
-// clocks of exponentials; alone, the two state warps a scheduler has at most: half of the time they wait for their own results.
+// What bounds it: with work for all SMs nothing alone.  A row of 32 channels (16 states) takes 66 clocks, of which the exponentials' pipe is busy for 40 and the
+// loads of 2 L + 32 words from shared memory take 40 to 50 beside it; 68 % of the issue slots are used, and warps wait most for the other kind at the
+// barriers.  Alone (4096 rows and channels), the two state warps a scheduler has at most, which wait for their own results: 61 % of the issue slots, 49 % of the pipe.
 //   SSM_WHOLE: the piece is the sequence      SSM_ENDS: the piece's state from zero, and the sum of its time steps
 //   SSM_PIECE: the piece from the state that the pieces before it leave
 constexpr int SSM_ROWS = 32, SSM_STATES = 128, SSM_HELP = 128, SSM_THREADS = SSM_STATES + SSM_HELP, SSM_RING = 4;
@@ -432,10 +434,15 @@ cudaError_t ssm_seq_split(const SsmArgs &a, const SeqTable &t, cudaStream_t st) 
   if (e == cudaSuccess) e = op_launch(ssm_join_kernel, dim3((unsigned)(((size_t)a.d * a.n + 255) / 256), t.n), 256, 0, st, 1, a, t);
   return e == cudaSuccess ? ssm_seq_mode<T, NS, L, 2, SSM_PIECE, VEC>(a, t, items, st) : e;
 }
-// States a lane.  Few channels and sequences: fewer states, more CTAs and the shorter chain (4096 rows of 768 channels with 16 states: 80 us with one a
-// lane, 107 with two, 185 with four; of 1536: 119, 107, 185; of 4096: 235, 167, 187; two sequences of 4096: 215, 167, 144; 1000 rows of
-// 2048 with 64: 84 with four a lane, 89 with eight; 4096 of 2048 with 8: 105 with one, 141 with two; of 4096: 144, 142).  Many: three
-// CTAs an SM where their registers allow it (11 sequences of 5120 channels 117 us against 127; one of 4096 198 against 187).
+// States a lane, CTAs an SM (fp16, us on the device, sequences whole).  Few channels and sequences: fewer states, more CTAs and the shorter chain:
+//   one sequence of 4096 rows, 16 states        1 a lane   2     4
+//     768 channels                                    79   106   184   (in pieces, four a lane: 67)
+//     1536                                           120   107   184
+//     4096                                           236   168   186
+//   two of 4096 rows in all, 4096 channels           216   169   140
+//   1000 rows of 2048, 64 states: 81 with four a lane, 88 with eight; 4096 of 2048, 8 states: 103 with one, 139 with two; of 4096: 143, 142.
+// Many: three CTAs an SM where their registers allow it (11 sequences, 3001 rows of 5120 channels 112 against 122), not where all CTAs find a place with two
+// (one of 4096 rows and channels, four a lane: 194 against 186).
 template <typename T, bool VEC>
 cudaError_t ssm_seq_any(const SsmArgs &a, const SeqTable &t, cudaStream_t st) {
   auto ctas = [&](int ch) { return (long long)((a.d / a.groups + ch - 1) / ch) * a.groups * t.n; };

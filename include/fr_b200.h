@@ -274,7 +274,7 @@ const char *fr_b200_op_last_error(void);
  * the streams' states (the reference has none of them; they stand beside its recurrences above).  Common to all:
  *   - tensors are [rows, width] pieces whose rows lie `ld` elements apart; dtype FR_B200_T_F16, _BF16 or _F32; parameters
  *     (bias, weights of the convolution, A, D, dt_bias) are fp32.  Sums, states and statistics are fp32, each output is
- *     rounded once.  No alignment beyond the element's is asked; rows and pointers of whole 16 bytes are faster.  Up to
+ *     rounded once.  No alignment beyond the element's is asked; rows and pointers of whole 16 bytes (of fp32 rows: 32) are faster.  Up to
  *     2^24 channels (2^23 of a scan);
  *   - asynchronous on `stream`, on `device` whatever device is current (the caller's stays current); nothing is allocated,
  *     nothing is synchronised, no result depends on the order of atomics: calls may be captured, and captured calls hold
@@ -282,7 +282,7 @@ const char *fr_b200_op_last_error(void);
  *   - waits inside fr_b200_linear's kernels are bounded.  Where one gives up (a fault of the device) the rows concerned hold NaN, also
  *     when a captured call is replayed, no other call is refused, and fr_b200_op_status() tells;
  *   - host arrays are checked: FR_B200_E_ARG, with the reason in fr_b200_op_last_error(), and nothing is launched.
- *     Outputs may not overlap inputs or the pool, except where it says so;
+ *     Outputs may not overlap inputs, parameters or the pool, except where it says so, nor the work area anything;
  *   - sequences: `starts` (host [n_seq + 1], not decreasing, within 0 .. rows) gives sequence i the rows starts[i] ..
  *     starts[i + 1] - 1, none allowed; NULL: one sequence of all rows.  Rows of no sequence stay as they were in `out`;
  *   - slots: the state of stream i is read from slot from[i] of the pool `state` (slots state_stride elements apart) and
