@@ -101,7 +101,7 @@ struct fr_b200_model {
   cudaStream_t seq_streams[4] = {nullptr, nullptr, nullptr, nullptr};   // long prompts: one stream per piece of rows
   std::vector<cudaEvent_t> seq_events;                                  // [piece][layer] + one start event
   // Once a step was captured: its graph goes on using the buffers that a later call outgrows (see grow()), and on reading the copy of the token-shift
-  // states that it was captured with (state_reset, state_copy).
+  // states that it was captured with (state_copy).
   bool captured = false;
   std::vector<void *> outgrown;
   // scratch for uploads
@@ -1512,11 +1512,10 @@ int fr_b200_state_reset(fr_b200_model *m, int slot) {
       for (int i = 0; i < m->C; ++i) pp[i] = -1e30f;
     }
   }
-  // (both copies of the token-shift states begin anew, so that the next token may read either; steps captured before read theirs)
   for (int s = 0; s < m->cfg.max_batch; ++s)
     if (slot < 0 || slot == s) {
       CU(cudaMemcpy(m->d_state + (size_t)s * m->state_stride, h.data(), per, cudaMemcpyHostToDevice));
-      if (!m->captured) m->par[s] = 0;
+      m->par[s] = 0;
     }
   return FR_B200_OK;
 }
@@ -1548,19 +1547,19 @@ int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_
     if (capturing(st)) return fail(FR_B200_E_STATE, "state_copy on a capturing stream: which copy of its token-shift states a slot reads is known to the host, and changes from token to token");
     CU(cudaSetDevice(m->device));
     // Both copies of the token-shift states move, and with them which one is read next, so that streams forked from one are decoded together as they
-    // are.  Where steps were captured a slot goes on reading the copy that it read (they do): if the source reads the other one, that is copied over.
+    // are.  Where steps were captured a slot goes on reading the copy that it read (they do), and both copies are what the source's next token reads.
     std::vector<unsigned> par(m->par);
     std::vector<int32_t> turned;
-    std::vector<uint8_t> reads;
+    std::vector<uint8_t> other;
     for (int i = 0; i < n; ++i) {
       if (!m->captured) par[dst[i]] = src[i] < 0 ? 0u : m->par[src[i]];
-      else if (src[i] >= 0 && m->par[src[i]] != m->par[dst[i]]) { turned.push_back(dst[i]); reads.push_back((uint8_t)m->par[dst[i]]); }
+      else if (src[i] >= 0 && src[i] != dst[i]) { turned.push_back(dst[i]); other.push_back((uint8_t)(1u - m->par[src[i]])); }
     }
     const SlotFill pp{off_mid(m->C, m->cfg.act_fp16) + 2 * (size_t)m->C * 4, m->layer_stride, m->L, m->C, -1e30f};
     CU(launch_slots_copy(m->d_state, m->layer_stride * m->L, m->state_stride, m->cfg.max_batch, n, src, dst, m->v5 ? nullptr : &pp, st));
     const int af = m->cfg.act_fp16;
     const SlotPairs shift{{off_sx(m->C, af, 0), off_ffn_sx(m->C, m->H, m->v5, af, 0)}, m->layer_stride, m->L, (int)(m->C * act_bytes(af) / 4)};
-    CU(launch_slots_turn(m->d_state, m->state_stride, (int)turned.size(), turned.data(), reads.data(), shift, st));
+    CU(launch_slots_turn(m->d_state, m->state_stride, (int)turned.size(), turned.data(), other.data(), shift, st));
     m->par.swap(par);
     if (m->cfg.host_visible_state) CU(cudaStreamSynchronize(st));
   } catch (const std::bad_alloc &) {

@@ -194,29 +194,38 @@ def test_captured_steps_go_on_from_copied_states(pkg, synth, version, fmt):
     m.close()
 
 
-@pytest.mark.parametrize("clear", ["reset", "copy"])
 @pytest.mark.parametrize("version", ["4", "5.2"])
-def test_captured_steps_go_on_from_cleared_states(pkg, synth, version, clear):
-    """a graph of two tokens whose first reads the second copy, replayed behind a reset: what the same tokens give outside it, and the step behind them"""
+def test_captured_steps_go_on_from_cleared_states(pkg, synth, version):
+    """a graph of two tokens, replayed behind streams that were cleared in the middle of a batch (the batch reads either copy), or reset as a whole behind
+    an odd number of tokens (then it reads the first): what the same tokens give outside it, and the step behind them"""
     shape = synth.Shape(version, 2, 128, 512, 96, n_head=2 if version != "4" else 0)
     m = pkg.Model(synth.to_file_dtypes(shape, synth.generate(shape, seed=11, ln_random=True), "fp16"), "cuda fp16", shape=shape, max_batch=2)
     ids = synth.token_ids(shape, 6, seed=9).reshape(3, 2).astype(np.int32)
-    want = np.stack([m.decode(ids[t]) for t in (0, 1, 2)])     # (an odd number of tokens: the next reads the second copy)
+    want = np.stack([m.decode(ids[t]) for t in (0, 1, 2)])
     after = [m.export_state(b) for b in (0, 1)]
     got = torch.zeros(2, 2, shape.vocab, device="cuda")
-    graph = _capture(pkg, lambda st: [pkg.lib().fr_b200_decode(m.handle, ids[t].ctypes.data_as(ctypes.c_void_p), 2,
-                                                               ctypes.c_void_p(got[t].data_ptr()), None, st) for t in (0, 1)])
-    for _ in range(2):
-        if clear == "reset":
-            m.reset_states()
-        else:
-            m.copy_states([-1, -1], [0, 1])
-        graph.replay()
+
+    def graph():
+        return _capture(pkg, lambda st: [pkg.lib().fr_b200_decode(m.handle, ids[t].ctypes.data_as(ctypes.c_void_p), 2, ctypes.c_void_p(got[t].data_ptr()), None, st)
+                                         for t in (0, 1)])
+
+    def replayed(g):
+        g.replay()
         torch.cuda.synchronize()
         assert np.array_equal(got.cpu().numpy(), want[:2])
         assert np.array_equal(m.decode(ids[2]), want[2])
         assert all(np.array_equal(m.export_state(b), after[b]) for b in (0, 1))
-        m.decode(ids[2])                                       # (an even number between the replays)
+
+    g = graph()                                    # (an odd number of tokens: it reads the second copy)
+    for _ in range(2):
+        m.copy_states([-1, -1], [0, 1])
+        replayed(g)
+        m.decode(ids[2])                           # (an even number between the replays)
+    m.reset_states()
+    g = graph()
+    for _ in range(2):
+        replayed(g)                                # (three tokens in all)
+        m.reset_states()
     m.close()
 
 
