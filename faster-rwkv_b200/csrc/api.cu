@@ -1546,14 +1546,15 @@ int fr_b200_state_copy(fr_b200_model *m, int n, const int32_t *src, const int32_
     if (int rc = check_moves(m->cfg.max_batch, n, src, dst)) return fail(rc, fr_b200_op_last_error());
     if (capturing(st)) return fail(FR_B200_E_STATE, "state_copy on a capturing stream: which copy of its token-shift states a slot reads is known to the host, and changes from token to token");
     CU(cudaSetDevice(m->device));
-    // Both copies of the token-shift states move, and with them which one is read next, so that streams forked from one are decoded together as they
-    // are.  Where steps were captured a slot goes on reading the copy that it read (they do), and both copies are what the source's next token reads.
+    // Both copies of the token-shift states move, and the destination is in step with stream 0, so that a batch is decoded as it lies.  Where the source
+    // is not, what its next token reads goes into the other copy, too; also once a step was captured: its graph may read either.
     std::vector<unsigned> par(m->par);
     std::vector<int32_t> turned;
     std::vector<uint8_t> other;
     for (int i = 0; i < n; ++i) {
-      if (!m->captured) par[dst[i]] = src[i] < 0 ? 0u : m->par[src[i]];
-      else if (src[i] >= 0 && src[i] != dst[i]) { turned.push_back(dst[i]); other.push_back((uint8_t)(1u - m->par[src[i]])); }
+      if (src[i] == dst[i]) continue;
+      par[dst[i]] = m->par[0];
+      if (src[i] >= 0 && (m->captured || m->par[src[i]] != m->par[0])) { turned.push_back(dst[i]); other.push_back((uint8_t)(1u - m->par[src[i]])); }
     }
     const SlotFill pp{off_mid(m->C, m->cfg.act_fp16) + 2 * (size_t)m->C * 4, m->layer_stride, m->L, m->C, -1e30f};
     CU(launch_slots_copy(m->d_state, m->layer_stride * m->L, m->state_stride, m->cfg.max_batch, n, src, dst, m->v5 ? nullptr : &pp, st));

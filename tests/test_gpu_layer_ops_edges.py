@@ -195,6 +195,37 @@ def test_captured_steps_go_on_from_copied_states(pkg, synth, version, fmt):
 
 
 @pytest.mark.parametrize("version", ["4", "5.2"])
+def test_a_batch_forked_from_a_stream_out_of_step_is_captured(pkg, synth, version):
+    """Streams of a batch take the state of one that has seen an odd number of tokens, beside others that have seen none; the batch is captured and replayed
+    twice: four steps like those outside a graph.  (A stream out of step would be brought into it by copies that every replay makes again.)"""
+    shape = synth.Shape(version, 2, 128, 512, 96, n_head=2 if version != "4" else 0)
+    tensors = synth.to_file_dtypes(shape, synth.generate(shape, seed=11, ln_random=True), "fp16")
+    m = pkg.Model(tensors, "cuda fp16", shape=shape, max_batch=5)
+    ids = synth.token_ids(shape, 8, seed=9).reshape(2, 4).astype(np.int32)
+    m.run([5, 9, 2])
+    prompt = m.export_state(0)
+    m.copy_states([0], [4])
+    m.reset_states(0)
+    m.copy_states([4, 4], [1, 3])
+    assert all(np.array_equal(m.export_state(b), prompt) for b in (1, 3, 4))
+    start = [m.export_state(b) for b in range(4)]
+    got = torch.zeros(2, 4, shape.vocab, device="cuda")
+    graph = _capture(pkg, lambda st: [pkg.lib().fr_b200_decode(m.handle, ids[t].ctypes.data_as(ctypes.c_void_p), 4, ctypes.c_void_p(got[t].data_ptr()), None, st)
+                                      for t in (0, 1)])
+    have = []
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        have.extend(got.cpu().numpy())
+    end = [m.export_state(b) for b in range(4)]
+    for b in range(4):
+        m.import_state(start[b], b)
+    assert np.array_equal(np.stack(have), np.stack([m.decode(ids[t]) for t in (0, 1, 0, 1)]))
+    assert all(np.array_equal(m.export_state(b), end[b]) for b in range(4))
+    m.close()
+
+
+@pytest.mark.parametrize("version", ["4", "5.2"])
 def test_captured_steps_go_on_from_cleared_states(pkg, synth, version):
     """a graph of two tokens, replayed behind streams that were cleared in the middle of a batch (the batch reads either copy), or reset as a whole behind
     an odd number of tokens (then it reads the first): what the same tokens give outside it, and the step behind them"""
